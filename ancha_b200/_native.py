@@ -18,6 +18,7 @@ PRECISION_F32, PRECISION_BF16, PRECISION_F16 = 0, 1, 2
 PRECISIONS = {"f32": PRECISION_F32, "bf16": PRECISION_BF16, "f16": PRECISION_F16}
 W_KN, W_NK = 0, 1
 ACT_NONE, ACT_GELU, ACT_TANH, ACT_GLU = 0, 1, 2, 3
+MXF8, MXF4, NVF4 = 0, 1, 2
 
 STATUS_NAMES = {OK: "ok", E_UNSUPPORTED: "unsupported", E_INVALID: "invalid", E_CUDA: "cuda",
                 E_CANCELLED: "cancelled", E_IO: "io", E_TIMEOUT: "timeout",
@@ -26,7 +27,8 @@ STATUS_NAMES = {OK: "ok", E_UNSUPPORTED: "unsupported", E_INVALID: "invalid", E_
 # Every symbol the header declares (checked by the CPU test suite).
 EXPORTS = ("ancha_last_error", "ancha_version", "ancha_available", "ancha_wait_selftest", "ancha_attention_fwd",
            "ancha_attention_workspace", "ancha_attention_fwd_ws", "ancha_linear_fwd", "ancha_linear_workspace",
-           "ancha_linear_fwd_ws", "ancha_stft_fwd", "ancha_istft_masked", "ancha_istft_masked_static", "ancha_ola_add",
+           "ancha_linear_fwd_ws", "ancha_mx_layout", "ancha_mx_quantize", "ancha_mx_dequantize",
+           "ancha_mx_add_rms_norm_fwd", "ancha_mx_linear_fwd", "ancha_stft_fwd", "ancha_istft_masked", "ancha_istft_masked_static", "ancha_ola_add",
            "ancha_model_load", "ancha_model_info", "ancha_model_forward", "ancha_model_free",
            "ancha_mdx23c_load", "ancha_mdx23c_info", "ancha_mdx23c_forward", "ancha_mdx23c_separate_pcm",
            "ancha_mdx23c_plan", "ancha_mdx23c_free", "ancha_mdx_graph_inspect", "ancha_mdx_load",
@@ -60,6 +62,21 @@ class LinearDesc(C.Structure):
                 ("ldw", C.c_int64), ("ldout", C.c_int64), ("ldres", C.c_int64),
                 ("act", C.c_int), ("rope_width", C.c_int), ("rope_tokens", C.c_int),
                 ("rope_div", C.c_int), ("row_scale", C.c_void_p)]
+
+
+class MxArray(C.Structure):
+    _fields_ = [("format", C.c_int), ("rows", C.c_int64), ("cols", C.c_int64), ("data", C.c_void_p),
+                ("ld", C.c_int64), ("scales", C.c_void_p), ("global_scale", C.c_void_p)]
+
+
+class MxNormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("residual_dtype", C.c_int), ("ldx", C.c_int64), ("ldres", C.c_int64),
+                ("ldres_out", C.c_int64), ("eps", C.c_double)]
+
+
+class MxLinearDesc(C.Structure):
+    _fields_ = [("act", C.c_int), ("out_dtype", C.c_int), ("residual_dtype", C.c_int), ("ldout", C.c_int64),
+                ("ldres", C.c_int64)]
 
 
 class SeparateOpts(C.Structure):
@@ -103,6 +120,12 @@ def lib() -> C.CDLL:
             "ancha_linear_fwd": (i32, [C.POINTER(LinearDesc), vp, vp, vp, vp, vp, vp, vp]),
             "ancha_linear_workspace": (i32, [C.POINTER(LinearDesc), C.POINTER(C.c_size_t)]),
             "ancha_linear_fwd_ws": (i32, [C.POINTER(LinearDesc), vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
+            "ancha_mx_layout": (i32, [i32, i64, i64, C.POINTER(i64), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+            "ancha_mx_quantize": (i32, [vp, i32, i64, C.POINTER(MxArray), vp]),
+            "ancha_mx_dequantize": (i32, [C.POINTER(MxArray), vp, i32, i64, vp]),
+            "ancha_mx_add_rms_norm_fwd": (i32, [C.POINTER(MxNormDesc), vp, vp, vp, vp, C.POINTER(MxArray), vp]),
+            "ancha_mx_linear_fwd": (i32, [C.POINTER(MxLinearDesc), C.POINTER(MxArray), C.POINTER(MxArray), vp, vp, vp,
+                                          C.POINTER(MxArray), vp]),
             "ancha_stft_fwd": (i32, [vp, i32, i32, i32, vp, vp]),
             "ancha_istft_masked": (i32, [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]),
             "ancha_istft_masked_static": (i32, [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp]),

@@ -17,6 +17,7 @@
 #include "gemm.cuh"
 #include "mdx23c_model.hpp"
 #include "mdx_exec.hpp"
+#include "mx.cuh"
 #include "onnx.hpp"
 #include "model.hpp"
 #include "tc.cuh"
@@ -82,6 +83,44 @@ int attention_args(const ancha_attn_desc* d, const void* q, const void* k, const
     a->q_col = d->q_col; a->k_col = d->k_col; a->v_col = d->v_col;
     a->gate_col = gate ? d->gate_col : 0; a->out_col = d->out_col;
     a->elt = d->dtype;
+    return ANCHA_OK;
+}
+
+bool float_type(int t) { return t == ANCHA_F32 || t == ANCHA_BF16 || t == ANCHA_F16; }
+
+bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+// The rules of ancha_mx_array; `who` opens the messages.
+int mx_shape(const std::string& who, int format, int64_t rows, int64_t cols) {
+    if (format != ANCHA_MXF8 && format != ANCHA_MXF4 && format != ANCHA_NVF4)
+        return fail(ANCHA_E_INVALID, who + ": unknown format");
+    if (rows < 0 || cols < 1) return fail(ANCHA_E_INVALID, who + ": empty rows or a negative shape");
+    if (rows > kMaxMxRows || cols > kMaxMxCols) return fail(ANCHA_E_UNSUPPORTED, who + ": array too large");
+    return ANCHA_OK;
+}
+
+int mx_array(const std::string& who, const ancha_mx_array* d, MxArray* a) {
+    if (!d) return fail(ANCHA_E_INVALID, who + ": null array");
+    ANCHA_TRY(mx_shape(who, d->format, d->rows, d->cols));
+    if (d->rows && (!d->data || !d->scales)) return fail(ANCHA_E_INVALID, who + ": null data or scales");
+    if (misaligned(d->data, 16) || misaligned(d->scales, 16) || d->ld % 16)
+        return fail(ANCHA_E_INVALID, who + ": data, scales and ld must be multiples of 16 bytes");
+    if (d->ld < mx_row_bytes(d->format, d->cols) || d->ld > kMaxMxLd)
+        return fail(ANCHA_E_INVALID, who + ": ld shorter than a row, or too large");
+    if (d->global_scale && d->format != ANCHA_NVF4)
+        return fail(ANCHA_E_INVALID, who + ": an array scale with a format that has none");
+    if (misaligned(d->global_scale, 4)) return fail(ANCHA_E_INVALID, who + ": array scale not 4-byte aligned");
+    *a = MxArray{d->format, d->rows, (int)d->cols, static_cast<uint8_t*>(d->data), d->ld,
+                 static_cast<uint8_t*>(d->scales), d->global_scale};
+    return ANCHA_OK;
+}
+
+// A plain matrix of `cols` columns: its type, row stride and element alignment.
+int mx_matrix(const std::string& who, const void* p, int dtype, int64_t ld, int64_t cols) {
+    if (!p) return fail(ANCHA_E_INVALID, who + ": null");
+    if (!float_type(dtype)) return fail(ANCHA_E_INVALID, who + ": unknown dtype");
+    if (ld < cols || ld > kMaxMxLd) return fail(ANCHA_E_INVALID, who + ": row stride shorter than a row, or too large");
+    if (misaligned(p, elt_size(dtype))) return fail(ANCHA_E_INVALID, who + ": not aligned to its elements");
     return ANCHA_OK;
 }
 }  // namespace
@@ -235,6 +274,93 @@ int ancha_linear_fwd_ws(const ancha_linear_desc* d, const void* x, const void* w
 int ancha_linear_fwd(const ancha_linear_desc* d, const void* x, const void* w, const float* bias,
                      const float* residual, const float* rope, void* out, void* stream) {
     return ancha_linear_fwd_ws(d, x, w, bias, residual, rope, out, nullptr, 0, stream);
+}
+
+int ancha_mx_layout(int format, int64_t rows, int64_t cols, int64_t* ld, size_t* data_bytes, size_t* scale_bytes) {
+    ANCHA_TRY(mx_shape("mx_layout", format, rows, cols));
+    const int64_t row = mx_row_bytes(format, cols);
+    if (ld) *ld = row;
+    if (data_bytes) *data_bytes = (size_t)(rows * row);
+    if (scale_bytes) *scale_bytes = (size_t)(ceil_div(rows, 128) * mx_ktiles(format, cols) * 512);
+    return ANCHA_OK;
+}
+
+int ancha_mx_quantize(const void* x, int dtype, int64_t ldx, const ancha_mx_array* out, void* stream) {
+    MxArray o;
+    ANCHA_TRY(mx_array("mx_quantize: out", out, &o));
+    if (!o.rows) return ANCHA_OK;
+    ANCHA_TRY(mx_matrix("mx_quantize: x", x, dtype, ldx, o.cols));
+    return mx_quantize(x, dtype, ldx, o, as_stream(stream));
+}
+
+int ancha_mx_dequantize(const ancha_mx_array* x, void* out, int dtype, int64_t ldout, void* stream) {
+    MxArray a;
+    ANCHA_TRY(mx_array("mx_dequantize: x", x, &a));
+    if (!a.rows) return ANCHA_OK;
+    ANCHA_TRY(mx_matrix("mx_dequantize: out", out, dtype, ldout, a.cols));
+    return mx_dequantize(a, out, dtype, ldout, as_stream(stream));
+}
+
+int ancha_mx_add_rms_norm_fwd(const ancha_mx_norm_desc* d, const void* x, const void* residual, const float* gain,
+                              void* residual_out, const ancha_mx_array* out, void* stream) {
+    if (!d) return fail(ANCHA_E_INVALID, "mx_add_rms_norm: null argument");
+    MxArray o;
+    ANCHA_TRY(mx_array("mx_add_rms_norm: out", out, &o));
+    if (!(d->eps > 0) || d->eps > 1e300) return fail(ANCHA_E_INVALID, "mx_add_rms_norm: eps must be a number > 0");
+    if (o.cols > kMaxNormCols) return fail(ANCHA_E_UNSUPPORTED, "mx_add_rms_norm: rows wider than 32768");
+    if (!o.rows) return ANCHA_OK;
+    ANCHA_TRY(mx_matrix("mx_add_rms_norm: x", x, d->dtype, d->ldx, o.cols));
+    if (residual) {
+        ANCHA_TRY(mx_matrix("mx_add_rms_norm: residual", residual, d->residual_dtype, d->ldres, o.cols));
+        if (!residual_out) return fail(ANCHA_E_INVALID, "mx_add_rms_norm: a residual without residual_out");
+    } else if (residual_out && d->residual_dtype != d->dtype) {
+        return fail(ANCHA_E_INVALID, "mx_add_rms_norm: without a residual the stream has the type of x");
+    }
+    if (residual_out) {
+        ANCHA_TRY(mx_matrix("mx_add_rms_norm: residual_out", residual_out, d->residual_dtype, d->ldres_out, o.cols));
+        if (residual_out == residual && d->ldres_out != d->ldres)
+            return fail(ANCHA_E_INVALID, "mx_add_rms_norm: residual_out over residual with another row stride");
+        if (residual_out == x && (d->ldres_out != d->ldx || d->residual_dtype != d->dtype))
+            return fail(ANCHA_E_INVALID, "mx_add_rms_norm: residual_out over x with another row stride or type");
+    }
+    if (misaligned(gain, 4)) return fail(ANCHA_E_INVALID, "mx_add_rms_norm: gain not 4-byte aligned");
+    return mx_add_rms_norm(x, d->dtype, d->ldx, residual, residual ? d->residual_dtype : d->dtype, d->ldres,
+                           residual_out, d->ldres_out, gain, d->eps, o, as_stream(stream));
+}
+
+int ancha_mx_linear_fwd(const ancha_mx_linear_desc* d, const ancha_mx_array* x, const ancha_mx_array* w,
+                        const float* bias, const void* residual, void* out, const ancha_mx_array* out_mx,
+                        void* stream) {
+    if (!d) return fail(ANCHA_E_INVALID, "mx_linear: null argument");
+    MxLinear q{};
+    ANCHA_TRY(mx_array("mx_linear: x", x, &q.x));
+    ANCHA_TRY(mx_array("mx_linear: w", w, &q.w));
+    if (q.x.format != q.w.format) return fail(ANCHA_E_INVALID, "mx_linear: x and w of two formats");
+    if (q.x.cols != q.w.cols) return fail(ANCHA_E_INVALID, "mx_linear: x and w of two depths");
+    if (q.w.rows < 1 || q.w.rows > kMaxMxCols) return fail(ANCHA_E_INVALID, "mx_linear: empty or too many weight rows");
+    if (d->act != ANCHA_ACT_NONE && d->act != ANCHA_ACT_GELU && d->act != ANCHA_ACT_TANH)
+        return fail(ANCHA_E_UNSUPPORTED, "mx_linear: activation not supported");
+    if (out && out_mx) return fail(ANCHA_E_INVALID, "mx_linear: out and out_mx exclude each other");
+    MxArray o;
+    if (out_mx) {
+        ANCHA_TRY(mx_array("mx_linear: out_mx", out_mx, &o));
+        if (o.rows != q.x.rows || o.cols != q.w.rows) return fail(ANCHA_E_INVALID, "mx_linear: out_mx of another shape");
+        q.out_mx = &o;
+    }
+    if (!q.x.rows) return ANCHA_OK;
+    if (!out && !out_mx) return fail(ANCHA_E_INVALID, "mx_linear: one of out and out_mx is needed");
+    if (out) ANCHA_TRY(mx_matrix("mx_linear: out", out, d->out_dtype, d->ldout, q.w.rows));
+    if (residual) {
+        ANCHA_TRY(mx_matrix("mx_linear: residual", residual, d->residual_dtype, d->ldres, q.w.rows));
+        if (residual == out && (d->ldres != d->ldout || d->residual_dtype != d->out_dtype))
+            return fail(ANCHA_E_INVALID, "mx_linear: out over the residual with another row stride or type");
+    }
+    if (misaligned(bias, 4)) return fail(ANCHA_E_INVALID, "mx_linear: bias not 4-byte aligned");
+    q.bias = bias;
+    q.residual = residual; q.res_type = d->residual_dtype; q.ldr = d->ldres;
+    q.act = d->act;
+    q.out = out; q.out_type = d->out_dtype; q.ldo = d->ldout;
+    return mx_linear(q, as_stream(stream));
 }
 
 int ancha_stft_fwd(const float* audio, int chunks, int samples, int hop, float* packed, void* stream) {

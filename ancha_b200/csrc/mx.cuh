@@ -1,0 +1,159 @@
+// Microscaled arrays: rows of 8-bit or 4-bit floating-point elements with one scale for each block
+// of consecutive elements of a row, and the device arithmetic that makes and expands them.
+//
+//   format       element        block  block scale                  array scale
+//   ANCHA_MXF8   E4M3 (8 bit)   32     E8M0, 2^(code - 127)         -
+//   ANCHA_MXF4   E2M1 (4 bit)   32     E8M0                         -
+//   ANCHA_NVF4   E2M1 (4 bit)   16     E4M3                         one f32 (device) or 1
+//
+// Elements lie row-major, `ld` bytes apart, the even column of a 4-bit pair in the low half of its
+// byte. Scales lie in the order in which the tensor cores take them: 512-byte tiles of 128 rows by
+// four blocks, tiles of one row range side by side,
+//   byte(row, block) = ((row / 128) * kt + block / 4) * 512 + (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4
+// with kt = ceil(blocks / 4). What a tile holds behind the last row or block is written as 0.
+#pragma once
+
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace ancha {
+
+enum : int { MXF8 = ANCHA_MXF8, MXF4 = ANCHA_MXF4, NVF4 = ANCHA_NVF4 };
+
+// Limits of an array: its coordinates are the tensor maps' 32-bit ones, and no byte count leaves 64 bits.
+constexpr int64_t kMaxMxRows = (int64_t(1) << 31) - 512, kMaxMxCols = (int64_t(1) << 31) - 512;
+constexpr int64_t kMaxMxLd = int64_t(1) << 32;  // rows apart: bytes of an array, elements of a matrix
+constexpr int kMaxNormCols = 32768;
+
+// A validated ancha_mx_array.
+struct MxArray {
+    int format;
+    int64_t rows;
+    int cols;
+    uint8_t* data;
+    int64_t ld;
+    uint8_t* scales;
+    const float* global_scale;  // device, NVF4 only; null = 1
+};
+
+__host__ __device__ constexpr int mx_block(int format) { return format == NVF4 ? 16 : 32; }
+// Bytes of `cols` elements.
+__host__ __device__ constexpr int64_t mx_bytes(int format, int64_t cols) {
+    return format == MXF8 ? cols : (cols + 1) / 2;
+}
+// Bytes of a row that are written: the elements and zeros up to a multiple of 16.
+__host__ __device__ constexpr int64_t mx_row_bytes(int format, int64_t cols) {
+    return (mx_bytes(format, cols) + 15) / 16 * 16;
+}
+// Scale tiles along a row.
+__host__ __device__ constexpr int64_t mx_ktiles(int format, int64_t cols) {
+    return (cols + 4 * mx_block(format) - 1) / (4 * mx_block(format));
+}
+
+struct MxLinear {
+    MxArray x, w;           // [m, k], [n, k], one format
+    const float* bias;      // [n] or null
+    const void* residual;   // [m, n] of res_type or null
+    int res_type;
+    int64_t ldr;
+    int act;                // ANCHA_ACT_NONE / GELU / TANH
+    void* out;              // [m, n] of out_type, or null with out_mx
+    int out_type;
+    int64_t ldo;
+    const MxArray* out_mx;  // [m, n] or null
+};
+
+int mx_quantize(const void* x, int dtype, int64_t ldx, const MxArray& out, cudaStream_t s);
+int mx_dequantize(const MxArray& x, void* out, int dtype, int64_t ldo, cudaStream_t s);
+int mx_add_rms_norm(const void* x, int dtype, int64_t ldx, const void* residual, int res_type, int64_t ldr,
+                    void* residual_out, int64_t ldro, const float* gain, double eps, const MxArray& out,
+                    cudaStream_t s);
+int mx_linear(const MxLinear& q, cudaStream_t s);
+
+#ifdef __CUDACC__
+
+// Offset of the 32-bit word that holds the scales of a row's blocks 4 kw .. 4 kw + 3.
+__device__ __forceinline__ int64_t mx_scale_word(int64_t row, int kw, int64_t kt) {
+    return ((row >> 7) * kt + kw) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+    const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3);
+    return __half2float(__half(h));
+}
+
+// 2^(code - 127); 255 is NaN and 0 the f32 subnormal 2^-127.
+__device__ __forceinline__ float e8m0_value(uint32_t code) {
+    return __uint_as_float(code == 255 ? 0x7FC00000u : code == 0 ? 0x00400000u : code << 23);
+}
+
+// The value a block's scale code stands for, without the array scale.
+template <int FMT>
+__device__ __forceinline__ float mx_scale_value(uint32_t code) {
+    return FMT == NVF4 ? e4m3_value(code) : e8m0_value(code);
+}
+
+// How a block is quantised: the code of its scale, and each element as v * mul (a power of two, exact)
+// or v / div (NVF4, whose divisor is no power of two: a division rounds next to a border of the grid as
+// the quotient does, a multiplication by the reciprocal does not). A block with an infinity or a NaN
+// has the scale NaN and elements 0; `live` is false for it, and where the divisor is 0.
+struct MxBlock {
+    uint32_t code;
+    float factor;
+    bool live;
+};
+
+// `amax_bits`: the largest of the block's |v| as f32 bits (as integers NaN > infinity > every number).
+// MX: the least power of two at which |v| max still rounds into the element's range, which for E4M3 is
+// up to 464 (a tie with the unrepresentable 480, to the even 448) and for E2M1 below 7. Rounding the
+// largest element down where that is its nearest value costs less than halving the resolution of the
+// rest: on normal data the rms error is 11.2 % for E2M1, against 11.5 % with the next power of two
+// from 6 on and 11.5 % with one power of two for all of [4, 8); 2.65 % for E4M3 (2.94 % for the latter).
+template <int FMT>
+__device__ __forceinline__ MxBlock mx_block_scale(uint32_t amax_bits, float global) {
+    MxBlock b;
+    const bool bad = amax_bits >= 0x7F800000u;
+    if (FMT == NVF4) {
+        const float s = bad ? 0.f : fminf(__uint_as_float(amax_bits) / (6.f * global), 448.f);
+        b.code = __nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
+        b.factor = e4m3_value(b.code) * global;
+        b.live = !bad && b.factor > 0.f;
+        if (bad) b.code = 0x7F;
+    } else {
+        const int field = (int)(amax_bits >> 23);
+        const uint32_t mantissa = amax_bits & 0x7FFFFFu;
+        const int top = FMT == MXF8 ? mantissa > 0x680000u : mantissa >= 0x600000u;
+        const int code = max(field - (FMT == MXF8 ? 8 : 2) + top, 0);
+        b.code = bad ? 255u : (uint32_t)code;
+        b.factor = __uint_as_float((uint32_t)(254 - code) << 23);
+        b.live = !bad;
+    }
+    return b;
+}
+
+template <int FMT>
+__device__ __forceinline__ float mx_scaled(float v, const MxBlock& b) {
+    if (!b.live) return 0.f;
+    return FMT == NVF4 ? __fdiv_rn(v, b.factor) : v * b.factor;
+}
+
+// Two elements: E4M3 codes in the two bytes of the result, or E2M1 codes in the two halves of one byte.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_pair(float lo, float hi) {
+    if (FMT == MXF8) return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+    return __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
+}
+template <int FMT>
+__device__ __forceinline__ float2 mx_pair_values(uint32_t code) {
+    const __half2_raw h = FMT == MXF8 ? __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code, __NV_E4M3)
+                                      : __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)code, __NV_E2M1);
+    return __half22float2(__half2(h));
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+#endif  // __CUDACC__
+
+}  // namespace ancha

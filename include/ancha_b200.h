@@ -160,6 +160,88 @@ ANCHA_API int ancha_linear_fwd_ws(const ancha_linear_desc* desc, const void* x, 
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------ *
+ * Microscaled operands: the linear of above in 8 and 4 bits (no reference counterpart)   *
+ * ------------------------------------------------------------------------------------ */
+
+/* Number formats of a row-major array. A block is a run of consecutive elements of a row; the last
+ * block of a row may be shorter.
+ *   ANCHA_MXF8  E4M3 elements (|max| 448), blocks of 32, scale 2^(code - 127) in 8 bits
+ *   ANCHA_MXF4  E2M1 elements (0, .5, 1, 1.5, 2, 3, 4, 6), blocks of 32, scale 2^(code - 127)
+ *   ANCHA_NVF4  E2M1 elements, blocks of 16, scale an E4M3 number, and one f32 scale of the array
+ * An element stands for element * block scale (* array scale). */
+enum { ANCHA_MXF8 = 0, ANCHA_MXF4 = 1, ANCHA_NVF4 = 2 };
+
+/* Such an array on the device. `data`: rows of `ld` bytes, one byte per element (ANCHA_MXF8) or two
+ * elements per byte, the even column in the low half. `scales`: tiles of 512 bytes for 128 rows by four
+ * blocks, kt = ceil(blocks per row / 4) of them side by side for each 128 rows; the scale of (row,
+ * block) is byte
+ *   ((row / 128) * kt + block / 4) * 512 + row % 32 * 16 + row % 128 / 32 * 4 + block % 4
+ * `data` and `scales` are 16-byte aligned and `ld` is a multiple of 16 (ancha_mx_layout gives the least).
+ * Calls that write an array write the element bytes of a row up to the next multiple of 16 and every
+ * byte of the scale tiles, with zeros behind the last column, row and block; data behind that, and rows
+ * behind `rows`, are left as they were. Calls that read one need the scales behind a row's last block to
+ * be numbers (not NaN: zeros). `global_scale`: the array scale, one device f32 > 0, or NULL for 1;
+ * ANCHA_NVF4 only. */
+typedef struct {
+    int format;
+    int64_t rows, cols;        /* rows >= 0, 1 <= cols < 2^31 - 512 */
+    void* data;
+    int64_t ld;
+    void* scales;
+    const float* global_scale;
+} ancha_mx_array;
+
+/* The least `ld` and the bytes of `data` (with that ld) and `scales` of an array. Any output pointer
+ * may be NULL. Host-only. */
+ANCHA_API int ancha_mx_layout(int format, int64_t rows, int64_t cols, int64_t* ld, size_t* data_bytes,
+                              size_t* scale_bytes);
+
+/* Quantise x[out->rows][out->cols] (`dtype` ANCHA_F32 / BF16 / F16, rows `ldx` elements apart) into `out`.
+ * Block scales: ANCHA_MXF8 / MXF4 the least power of two (from 2^-127 on) at which the block's largest
+ * magnitude rounds to a finite element; ANCHA_NVF4 that magnitude / (6 * array scale) rounded to E4M3, at
+ * most 448. Elements: value / scale rounded to nearest, ties to even, saturated; 0 where the scale is 0.
+ * A block that holds an infinity or a NaN gets the scale NaN and elements 0, so it expands to NaN. */
+ANCHA_API int ancha_mx_quantize(const void* x, int dtype, int64_t ldx, const ancha_mx_array* out, void* stream);
+
+/* Expand x into out[x->rows][x->cols] of `dtype` (rows `ldout` elements apart): element * scale, each
+ * product in f32, rounded once to dtype. */
+ANCHA_API int ancha_mx_dequantize(const ancha_mx_array* x, void* out, int dtype, int64_t ldout, void* stream);
+
+/* Operands of ancha_mx_add_rms_norm_fwd; sizes are those of its output array. */
+typedef struct {
+    int dtype, residual_dtype;    /* ANCHA_F32 / BF16 / F16 of x; of residual and residual_out */
+    int64_t ldx, ldres, ldres_out; /* rows, in elements                                        */
+    double eps;                   /* > 0                                                       */
+} ancha_mx_norm_desc;
+
+/* s = residual + x, rounded to residual_dtype and written to residual_out; out = the quantised rows of
+ * s / sqrt(mean(s^2) + eps) * gain. `residual` NULL: s = x (then residual_dtype = dtype), written to
+ * residual_out unless that is NULL too. gain: device f32 [cols] or NULL for 1. residual_out may be
+ * residual or x itself, with the same row stride and type; any other overlap is undefined. Rows of at most
+ * 32768 columns. The mean is taken with errors far below f32's, so a row's codes do not depend on how
+ * the kernel splits it. The norm of the reference's blocks (roformer.rs:16-24) is this one with
+ * gain = gamma, eps ~ 0. */
+ANCHA_API int ancha_mx_add_rms_norm_fwd(const ancha_mx_norm_desc* desc, const void* x, const void* residual,
+                                        const float* gain, void* residual_out, const ancha_mx_array* out,
+                                        void* stream);
+
+typedef struct {
+    int act;                  /* ANCHA_ACT_NONE / GELU / TANH                                  */
+    int out_dtype;            /* ANCHA_F32 / BF16 / F16 of out                                 */
+    int residual_dtype;       /* ANCHA_F32 / BF16 / F16 of residual                            */
+    int64_t ldout, ldres;     /* rows, in elements                                             */
+} ancha_mx_linear_desc;
+
+/* y[m, n] = act(sum_k x[m, k] * w[n, k] + bias[n]) + residual[m, n] for x [m, k] and w [n, k] of one
+ * format (ancha_linear_fwd's ANCHA_W_NK layout and order of the epilogue), on the block-scaled tensor
+ * cores with f32 accumulation. y is written to out (out_dtype), or quantised into out_mx (any format):
+ * exactly one of the two. bias: device f32 [n] or NULL; residual may be NULL, or out itself with the same
+ * type and row stride. No allocation, no workspace. */
+ANCHA_API int ancha_mx_linear_fwd(const ancha_mx_linear_desc* desc, const ancha_mx_array* x, const ancha_mx_array* w,
+                                  const float* bias, const void* residual, void* out, const ancha_mx_array* out_mx,
+                                  void* stream);
+
+/* ------------------------------------------------------------------------------------ *
  * Spectral DSP (replaces crates/ancha-audio/src/dsp.rs and chunk.rs on the device)     *
  * ------------------------------------------------------------------------------------ */
 
