@@ -1,113 +1,582 @@
-// Product of two microscaled arrays with bias, activation and residual.
+// Product of two microscaled arrays on the block-scaled tensor cores: y = act(x · wᵀ · g + bias) +
+// residual, x [m, k], w [n, k], f32 accumulation, y in 32 or 16 bits or quantised again.
+//
+// The scales need no arithmetic here: tcgen05.mma (kind mxf8f6f4 / mxf4 / mxf4nvf4, block_scale) takes a
+// 32-byte K step of both operands from shared memory and their block scales from TMEM, where tcgen05.cp
+// puts them 512 bytes (128 rows by 4 blocks) at a time; the stored order of the scales is the order that
+// copy wants. One K slab is 128 bytes of a row in every format (128 elements of 8 bits, 256 of 4), four
+// instructions; it needs 1 (mxf8), 2 (mxf4) or 4 (nvf4) scale tiles per 128 rows.
+//
+// Persistent and warp-specialised, as the 16-bit GEMM: warp 0 loads slabs of both operands and their
+// scales by TMA through a ring of stages, warp 1 issues the copies and products, the other warps drain
+// the accumulator. A CTA pair shares a 256 x 256 tile (each CTA holds 128 rows of x, half of w's rows, and
+// all of w's scales).
 #include "mx.cuh"
 #include "tc.cuh"
+
+#include <algorithm>
 
 namespace ancha {
 namespace {
 
-constexpr int T = 64, TK = 32;  // output tile and K step
+constexpr int BM = 128, SLAB = 128;          // rows of a CTA's tile, bytes of a K slab
+constexpr int OPERAND_BYTES = BM * SLAB;     // 128 rows of a slab
+constexpr int SF_TILE = 512;                 // a scale tile
+constexpr int EPI = 8;                       // epilogue warps
+constexpr int THREADS = 64 + 32 * EPI;
+constexpr int STAGING = 4096;                // per epilogue warp: 32 rows x 128 bytes
+// TMEM: two accumulators, then the scales of the slab in work.
+constexpr uint32_t SFA_COL = 448, SFB_COL = 464, TMEM_COLS = 512;
 
-template <int FMT>
-__device__ __forceinline__ float element(const MxArray& a, int64_t row, int col, int64_t kt, float g) {
-    if (row >= a.rows || col >= a.cols) return 0.f;
-    const uint8_t byte = a.data[row * a.ld + (FMT == MXF8 ? col : col / 2)];
-    const float e = FMT == MXF8 ? e4m3_value(byte)
-                                : (col % 2 ? mx_pair_values<FMT>(byte).y : mx_pair_values<FMT>(byte).x);
-    const int b = col / mx_block(FMT);
-    return e * mx_scale_value<FMT>(a.scales[mx_scale_word(row, b / 4, kt) + b % 4]) * g;
+constexpr int sf_tiles(int fmt) { return fmt == MXF8 ? 1 : fmt == MXF4 ? 2 : 4; }
+
+template <int FMT, int BN, bool PAIR>
+struct Shape {
+    static constexpr int SF = sf_tiles(FMT);
+    static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // w's rows in this CTA
+    static constexpr int B_BYTES = B_ROWS * SLAB;
+    static constexpr int SFA_BYTES = SF * SF_TILE, SFB_BYTES = SF * SF_TILE * (BN / 128);
+    static constexpr int STAGE = OPERAND_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+    static constexpr int STAGES = (227 * 1024 - 1024 - 256 - EPI * STAGING) / STAGE < 6
+                                      ? (227 * 1024 - 1024 - 256 - EPI * STAGING) / STAGE : 6;
+    static constexpr int BYTES = 1024 + STAGES * STAGE + EPI * STAGING + 256;
+    // Second accumulator. Two of 256 columns and the scales do not fit 512: they share 64 columns, which
+    // the epilogue of a tile drains first, so the next tile's products start when those are free.
+    static constexpr uint32_t ACC1 = BN == 256 ? 192 : BN;
+    static constexpr bool SHARED_COLS = BN == 256;
+};
+
+struct Params {
+    int m, n, kbytes;          // kbytes: bytes of a row of x or w that hold elements
+    int m_tiles, n_tiles, tiles;
+    const float* gx;           // array scales (NVF4) or null
+    const float* gw;
+    const float* bias;
+    const void* residual;
+    int64_t ldr;
+    int res_type, res_vec, act;
+    void* out;
+    int64_t ldo;
+    int out_type, out_mode;    // OUT_*
+    MxArray om;
+    int okt;                   // scale tiles along a row of om
+    int* err;
+};
+enum : int { OUT_TMA = 0, OUT_PLAIN = 1, OUT_MX = 2 };
+
+// ---- block-scaled tcgen05 -------------------------------------------------------------------
+
+// Scale-tile descriptor: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
 }
 
+// A scale tile into four TMEM columns, the same 32 lanes for each of the four lane quarters.
+template <bool PAIR>
+__device__ __forceinline__ void sf_copy(uint32_t tmem, uint64_t desc) {
+    if (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
+#define ANCHA_MX_MMA(GROUP, KIND)                                                                       \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                      \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" \
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)              \
+                 : "memory")
+
+template <int FMT, bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                    uint32_t accumulate) {
+    if (PAIR) {
+        if (FMT == MXF8) ANCHA_MX_MMA("2", "mxf8f6f4.block_scale.scale_vec::1X");
+        else if (FMT == MXF4) ANCHA_MX_MMA("2", "mxf4.block_scale.scale_vec::2X");
+        else ANCHA_MX_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else {
+        if (FMT == MXF8) ANCHA_MX_MMA("1", "mxf8f6f4.block_scale.scale_vec::1X");
+        else if (FMT == MXF4) ANCHA_MX_MMA("1", "mxf4.block_scale.scale_vec::2X");
+        else ANCHA_MX_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    }
+}
+#undef ANCHA_MX_MMA
+
+// Instruction descriptor without the scale byte selectors: element types (E4M3 is 0 of mxf8f6f4, E2M1 is 1 of
+// mxf4 / mxf4nvf4), N / 8 at bit 17, scale type E8M0 at bit 23, M / 128 at bit 27, both operands K-major.
 template <int FMT>
-__device__ __forceinline__ void quantize_row(const MxArray& o, const float* v, int64_t row, int c, int64_t kt) {
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n) {
+    return (FMT == MXF8 ? 0u : 1u << 7 | 1u << 10) | (uint32_t)(n >> 3) << 17 | (FMT == NVF4 ? 0u : 1u << 23) |
+           (uint32_t)(m >> 7) << 27;
+}
+
+// The products of one slab: `steps` (1 to 4) K steps of 32 bytes. Step i takes scale tile i / (4 / SF) and in
+// it the byte (1X), byte pair (2X) or all four bytes (4X) of its blocks.
+template <int FMT, bool PAIR, int BN>
+__device__ __forceinline__ void slab_products(uint32_t acc, uint32_t tmem, uint32_t a, uint32_t b, uint32_t sa,
+                                              uint32_t sb, uint32_t idesc, int steps, bool first) {
+    constexpr int SF = sf_tiles(FMT), PER = 4 / SF;  // K steps per scale tile
+#pragma unroll
+    for (int t = 0; t < SF; ++t) {
+        if (t * PER >= steps) break;
+        sf_copy<PAIR>(tmem + SFA_COL + 4 * t, sf_desc(sa + t * SF_TILE));
+#pragma unroll
+        for (int q = 0; q < BN / 128; ++q)
+            sf_copy<PAIR>(tmem + SFB_COL + t * (BN / 32) + 4 * q, sf_desc(sb + (q * SF + t) * SF_TILE));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i >= steps) break;
+        const int t = i / PER;
+        const uint32_t id = FMT == MXF8 ? i : FMT == MXF4 ? i % 2 * 2 : 0;
+        mma<FMT, PAIR>(acc, umma_desc_sw128(a + i * 32), umma_desc_sw128(b + i * 32), idesc | id << 4 | id << 29,
+                       tmem + SFA_COL + 4 * t, tmem + SFB_COL + t * (BN / 32), !(first && i == 0));
+    }
+}
+
+// ---- epilogue -------------------------------------------------------------------------------
+
+// GELU(x) = max(x, 0) - |x| Phi(-|x|) with Phi(-u) = 2^R(u), u = min(|x|, 5.5), R a polynomial in
+// v = u 2/5.5 - 1 of degree 9, fitted here to log2 Phi(-u) with the weight u Phi(-u) of the result (Lawson's
+// iteration). Evaluated in f32 its error is f32's: rms 3.9e-8 on [-4, 4], 2.4e-7 at most; the degree 7 fit of
+// the 16-bit epilogues (7e-7) moves the codes of a quantised output more often than the sum's own rounding.
+__device__ __forceinline__ void gelu2(float& x0, float& x1) {
+    constexpr float C[10] = {
+        -8.390586853027344f, -12.107649803161621f, -5.0239338874816895f, -0.18306505680084229f, 0.07878392934799194f,
+        -0.030920876190066338f, 0.009299345314502716f, -0.005405102390795946f, 0.0013578912476077676f, 0.001960539724677801f};
+    const uint64_t v = ffma2(f2(fminf(fabsf(x0), 5.5f), fminf(fabsf(x1), 5.5f)), f2(2.0f / 5.5f, 2.0f / 5.5f), f2(-1.0f, -1.0f));
+    uint64_t r = f2(C[9], C[9]);
+#pragma unroll
+    for (int i = 8; i >= 0; --i) r = ffma2(r, v, f2(C[i], C[i]));
+    float r0, r1;
+    f2_split(r, r0, r1);
+    x0 = fmaf(-fabsf(x0), ex2_approx(r0), fmaxf(x0, 0.f));
+    x1 = fmaf(-fabsf(x1), ex2_approx(r1), fmaxf(x1, 0.f));
+}
+
+__device__ __forceinline__ float residual_at(const Params& p, int64_t i) {
+    return p.res_type == ELT_F32    ? static_cast<const float*>(p.residual)[i]
+           : p.res_type == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[i])
+                                    : __half2float(static_cast<const __half*>(p.residual)[i]);
+}
+
+// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them).
+__device__ __forceinline__ void finish32(const Params& p, int64_t row, bool live, int c0, int nv, float alpha,
+                                         const uint32_t (&r)[32], float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
+    if (p.bias) {
+        if (nv == 32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(p.bias + c0 + j);
+                v[j] += q.x; v[j + 1] += q.y; v[j + 2] += q.z; v[j + 3] += q.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j < nv) v[j] += p.bias[c0 + j];
+        }
+    }
+    if (p.act == ANCHA_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) gelu2(v[j], v[j + 1]);
+    } else if (p.act == ANCHA_ACT_TANH) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) tanh_fast2(v[j], v[j + 1]);
+    }
+    if (p.residual && live) {
+        const int64_t at = row * p.ldr + c0;
+        if (p.res_vec && nv == 32) {
+            if (p.res_type == ELT_F32) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at + j);
+                    v[j] += q.x; v[j + 1] += q.y; v[j + 2] += q.z; v[j + 3] += q.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at + j);
+                    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = p.res_type == ELT_BF16
+                                             ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]))
+                                             : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                        v[j + 2 * i] += f.x;
+                        v[j + 2 * i + 1] += f.y;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (j < nv) v[j] += residual_at(p, at + j);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (j >= nv) v[j] = 0.f;
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
+    if (type == ELT_BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// A lane's row of 32 values in the swizzled staging layout of the TMA store (128-byte rows of f32 with the
+// 128-byte swizzle, 64-byte rows of 16 bits with the 64-byte swizzle).
+__device__ __forceinline__ void stage_row(uint8_t* buf, int lane, int type, const float (&v)[32]) {
+    if (type == ELT_F32) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) =
+                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
+                make_uint4(pack16(v[8 * q], v[8 * q + 1], type), pack16(v[8 * q + 2], v[8 * q + 3], type),
+                           pack16(v[8 * q + 4], v[8 * q + 5], type), pack16(v[8 * q + 6], v[8 * q + 7], type));
+    }
+}
+
+// Outputs that a TMA store cannot reach (odd addresses or strides): transposed through shared memory so that
+// a warp writes 32 neighbouring columns of a row at a time.
+__device__ __forceinline__ void store_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane,
+                                            const float (&v)[32]) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
+    __syncwarp();
+    if (lane >= nv) return;
+    for (int r = 0; r < 32 && row0 + r < p.m; ++r)
+        store_elt(p.out, (row0 + r) * p.ldo + c0 + lane, buf[r * 32 + (lane ^ r)], p.out_type);
+}
+
+// A lane's 32 columns quantised: one block of 32, or two of 16, in its registers.
+template <int FMT>
+__device__ __forceinline__ void store_mx(const MxArray& o, int okt, int64_t row, int c0, const float (&v)[32]) {
     constexpr int B = mx_block(FMT);
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
-    uint32_t a = 0;
-    for (int j = 0; j < B; ++j) a = max(a, abs_bits(v[j]));
-    const MxBlock b = mx_block_scale<FMT>(a, g);
-    for (int j = 0; j < B; j += 2) {
-        const uint32_t p = mx_pair<FMT>(mx_scaled<FMT>(v[j], b), mx_scaled<FMT>(v[j + 1], b));
-        const int64_t at = mx_bytes(FMT, c + j);
-        if (at >= mx_row_bytes(FMT, o.cols)) continue;
-        o.data[row * o.ld + at] = (uint8_t)p;
-        if (FMT == MXF8) o.data[row * o.ld + at + 1] = (uint8_t)(p >> 8);
+    uint32_t codes = 0, w[8];
+#pragma unroll
+    for (int h = 0; h < 32 / B; ++h) {
+        uint32_t a = 0;
+#pragma unroll
+        for (int j = 0; j < B; ++j) a = max(a, abs_bits(v[h * B + j]));
+        const MxBlock b = mx_block_scale<FMT>(a, g);
+        codes |= b.code << (8 * h);
+#pragma unroll
+        for (int j = 0; j < B; j += 2) {
+            const uint32_t q = mx_pair<FMT>(mx_scaled<FMT>(v[h * B + j], b), mx_scaled<FMT>(v[h * B + j + 1], b));
+            const int at = h * B + j;
+            if (FMT == MXF8) w[at / 4] = at % 4 ? w[at / 4] | q << 16 : q;
+            else w[at / 8] = at % 8 ? w[at / 8] | q << (at % 8 * 4) : q;
+        }
     }
-    o.scales[mx_scale_word(row, c / B / 4, kt) + c / B % 4] = (uint8_t)b.code;
+    uint8_t* d = o.data + row * o.ld + mx_bytes(FMT, c0);
+    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (FMT == MXF8 && c0 + 16 < o.cols) *reinterpret_cast<uint4*>(d + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    uint8_t* s = o.scales + mx_scale_word(row, c0 / B / 4, okt) + c0 / B % 4;
+    if (B == 32) *s = (uint8_t)codes;
+    else *reinterpret_cast<uint16_t*>(s) = (uint16_t)codes;
+}
+
+// Scales of a chunk that lies behind the last row or column, inside the last scale tiles: 0.
+__device__ __forceinline__ void zero_scales(const Params& p, int64_t row, int c0) {
+    const int b = mx_block(p.om.format);
+    if (row >= ((int64_t)p.m + 127) / 128 * 128 || c0 / (4 * b) >= p.okt) return;
+    uint8_t* s = p.om.scales + mx_scale_word(row, c0 / b / 4, p.okt) + c0 / b % 4;
+    if (b == 32) *s = 0;
+    else *reinterpret_cast<uint16_t*>(s) = 0;
+}
+
+template <int FMT, int BN, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1)
+linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+              const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
+              const __grid_constant__ CUtensorMap tout, const __grid_constant__ Params p) {
+    using S = Shape<FMT, BN, PAIR>;
+    constexpr int BMT = PAIR ? 2 * BM : BM, STAGES = S::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* a_tiles = smem;
+    uint8_t* b_tiles = a_tiles + STAGES * OPERAND_BYTES;
+    uint8_t* staging = b_tiles + STAGES * S::B_BYTES;  // 1024-byte aligned, as the operands
+    uint8_t* sa_tiles = staging + EPI * STAGING;
+    uint8_t* sb_tiles = sa_tiles + STAGES * S::SFA_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + STAGES * S::SFB_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* tfull = empty + STAGES;   // [2] accumulator ready
+    uint64_t* tempty = tfull + 2;       // [2] accumulator drained (with shared columns: [0], those drained)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    const int tile0 = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x;
+    const int tstep = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], PAIR ? 2 * EPI : EPI);
+        }
+        *abort = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+        prefetch_tma(&ta);
+        prefetch_tma(&tb);
+        prefetch_tma(&tsa);
+        prefetch_tma(&tsb);
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            tmem_alloc_pair(tmem_slot, TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, TMEM_COLS);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // the peer's barriers exist before anything arrives on them
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int slabs = (p.kbytes + SLAB - 1) / SLAB;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int t = tile0; t < p.tiles && !*abort; t += tstep) {
+                const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
+                for (int kb = 0; kb < slabs; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+                    uint8_t* a = a_tiles + s * OPERAND_BYTES;
+                    uint8_t* b = b_tiles + s * S::B_BYTES;
+                    uint8_t* sa = sa_tiles + s * S::SFA_BYTES;
+                    uint8_t* sb = sb_tiles + s * S::SFB_BYTES;
+                    if (PAIR) {
+                        // Both CTAs' copies complete on the even CTA's barrier, which expects both.
+                        const uint32_t fb = mapa_shared(smem_u32(&full[s]), 0);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::STAGE);
+                        tma_load_3d_pair(a, &ta, fb, kb * SLAB, m0 + (int)rank * BM, 0);
+                        tma_load_3d_pair(b, &tb, fb, kb * SLAB, n0 + (int)rank * S::B_ROWS, 0);
+                        tma_load_3d_pair(sa, &tsa, fb, 0, kb * S::SF * 2, m0 / 128 + (int)rank);
+                        tma_load_3d_pair(sb, &tsb, fb, 0, kb * S::SF * 2, n0 / 128);
+                    } else {
+                        mbar_arrive_expect_tx(&full[s], S::STAGE);
+                        tma_load_3d(a, &ta, &full[s], kb * SLAB, m0, 0);
+                        tma_load_3d(b, &tb, &full[s], kb * SLAB, n0, 0);
+                        tma_load_3d(sa, &tsa, &full[s], 0, kb * S::SF * 2, m0 / 128);
+                        tma_load_3d(sb, &tsb, &full[s], 0, kb * S::SF * 2, n0 / 128);
+                    }
+                }
+            }
+            if (*abort && rank == 0) {  // let copies in flight land before the CTA exits (bounded)
+                const long long c0 = clock64();
+                for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
+                    while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
+                    }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_of<FMT>(BMT, BN);
+            uint32_t it = 0, local = 0;
+            for (int t = tile0; t < p.tiles && !*abort; t += tstep, ++local) {
+                const int b = local & 1;
+                if (S::SHARED_COLS) {
+                    if (local && !mbar_wait(&tempty[0], (local - 1) & 1, abort, p.err)) break;
+                } else if (!mbar_wait(&tempty[b], ((local >> 1) & 1) ^ 1, abort, p.err)) {
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem + b * S::ACC1;
+                for (int kb = 0; kb < slabs; ++kb, ++it) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
+                    tc_fence_after();
+                    const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
+                    slab_products<FMT, PAIR, BN>(acc, tmem, smem_u32(a_tiles + s * OPERAND_BYTES),
+                                                 smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
+                                                 smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0);
+                    if (PAIR) umma_commit_pair(&empty[s], 0x3);
+                    else umma_commit(&empty[s]);
+                }
+                if (PAIR) umma_commit_pair(&tfull[b], 0x3);
+                else umma_commit(&tfull[b]);
+            }
+        }
+    } else {
+        constexpr int PER_QUARTER = EPI / 4, CHUNKS = BN / 32;
+        const int quarter = warp % 4, first = (warp - 2) / 4;
+        uint8_t* stage = staging + (warp - 2) * STAGING;
+        float alpha = 1.f;
+        if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
+        uint32_t local = 0;
+        bool stored = false;
+        for (int t = tile0; t < p.tiles; t += tstep, ++local) {
+            const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
+            const int b = local & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], (local >> 1) & 1, abort, p.err))) break;
+            tc_fence_after();
+            const int64_t row0 = m0 + (int)rank * BM + quarter * 32, row = row0 + lane;
+            const bool live = row < p.m;
+            const uint32_t base = tmem + b * S::ACC1 + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int o = first; o < CHUNKS; o += PER_QUARTER) {
+                // The shared columns, the last two chunks of one accumulator and the first two of the other, first.
+                const int col = 32 * (S::SHARED_COLS && b == 0 ? (o + CHUNKS - 2) % CHUNKS : o);
+                uint32_t r[32];
+                tmem_ld32(base + col, r);
+                tmem_wait_ld();
+                if (S::SHARED_COLS ? o == first : o + PER_QUARTER >= CHUNKS) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
+                        if (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0));
+                        else mbar_arrive(bar);
+                    }
+                }
+                const int c0 = n0 + col, nv = min(32, p.n - c0);
+                if (nv <= 0 || row0 >= p.m) {
+                    if (p.out_mode == OUT_MX) zero_scales(p, row, c0);
+                    continue;
+                }
+                float v[32];
+                finish32(p, row, live, c0, nv, alpha, r, v);
+                if (p.out_mode == OUT_TMA) {
+                    if (stored) {  // the store that last read this buffer is done with it
+                        if (lane == 0) bulk_wait_read<0>();
+                        __syncwarp();
+                    }
+                    stage_row(stage, lane, p.out_type, v);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&tout, stage, c0, (int)row0, 0);
+                        bulk_commit();
+                    }
+                    stored = true;
+                } else if (p.out_mode == OUT_PLAIN) {
+                    store_plain(p, reinterpret_cast<float*>(stage), row0, c0, nv, lane, v);
+                } else if (!live) {
+                    zero_scales(p, row, c0);
+                } else if (p.om.format == MXF8) {
+                    store_mx<MXF8>(p.om, p.okt, row, c0, v);
+                } else if (p.om.format == MXF4) {
+                    store_mx<MXF4>(p.om, p.okt, row, c0, v);
+                } else {
+                    store_mx<NVF4>(p.om, p.okt, row, c0, v);
+                }
+            }
+        }
+        if (lane == 0) bulk_wait<0>();
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    // With a pair, neither CTA releases TMEM or exits while the other may still use its shared memory.
+    if (PAIR) cluster_sync();
+    if (warp == 1) {
+        __syncwarp();
+        if (PAIR) tmem_dealloc_pair(tmem, TMEM_COLS);
+        else tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+template <int FMT, int BN, bool PAIR>
+int launch(const MxLinear& q, Params p, cudaStream_t s) {
+    using S = Shape<FMT, BN, PAIR>;
+    auto kernel = linear_kernel<FMT, BN, PAIR>;
+    static int slots[64] = {};  // co-resident CTAs (one per SM) or CTA pairs
+    int dev = 0;
+    ANCHA_CUDA(cudaGetDevice(&dev));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    if (!slots[dev & 63]) {
+        ANCHA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+        int n = 0;
+        if (PAIR) {
+            cfg.gridDim = dim3(2, 1, 1);
+            ANCHA_CUDA(cudaOccupancyMaxActiveClusters(&n, (void*)kernel, &cfg));
+            if (n < 1) return fail(ANCHA_E_UNSUPPORTED, "mx_linear: no CTA pair fits an SM pair");
+        } else {
+            ANCHA_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        }
+        slots[dev & 63] = n;
+    }
+    CUtensorMap ta, tb, tsa, tsb, to;
+    const int64_t akt = mx_ktiles(FMT, q.x.cols);
+    ANCHA_TRY(make_tma_bytes(&ta, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, BM, true));
+    ANCHA_TRY(make_tma_bytes(&tb, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, S::B_ROWS, true));
+    ANCHA_TRY(make_tma_scales(&tsa, q.x.scales, akt, ceil_div(p.m, 128), S::SF, 1));
+    ANCHA_TRY(make_tma_scales(&tsb, q.w.scales, akt, ceil_div(p.n, 128), S::SF, BN / 128));
+    to = ta;
+    if (p.out_mode == OUT_TMA)
+        ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, 32, 32));
+    p.m_tiles = (int)ceil_div(p.m, PAIR ? 2 * BM : BM);
+    p.n_tiles = (int)ceil_div(p.n, BN);
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    if (tiles > 0x7fffffff) return fail(ANCHA_E_UNSUPPORTED, "mx_linear: too many tiles");
+    p.tiles = (int)tiles;
+    const int units = std::min(p.tiles, slots[dev & 63]);
+    cfg.gridDim = dim3(PAIR ? 2 * units : units, 1, 1);
+    cfg.stream = s;
+    ANCHA_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, p));
+    return check_launch("mx_linear");
 }
 
 template <int FMT>
-__global__ void __launch_bounds__(256) linear_kernel(MxLinear q, MxArray om, bool mx_out) {
-    __shared__ float a[TK][T + 1], b[TK][T + 1], o[T][T + 1];
-    const int64_t m0 = (int64_t)blockIdx.y * T;
-    const int n0 = blockIdx.x * T, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int k = q.x.cols;
-    const int64_t kt = mx_ktiles(FMT, k);
-    const float gx = FMT == NVF4 && q.x.global_scale ? *q.x.global_scale : 1.f;
-    const float gw = FMT == NVF4 && q.w.global_scale ? *q.w.global_scale : 1.f;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < k; k0 += TK) {
-        for (int i = threadIdx.x; i < T * TK; i += 256) {
-            const int r = i / TK, c = i % TK;
-            a[c][r] = element<FMT>(q.x, m0 + r, k0 + c, kt, gx);
-            b[c][r] = element<FMT>(q.w, n0 + r, k0 + c, kt, gw);
-        }
-        __syncthreads();
-        for (int c = 0; c < TK; ++c)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[c][ty * 4 + i], b[c][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t row = m0 + ty * 4 + i;
-            const int col = n0 + tx * 4 + j;
-            float v = acc[i][j];
-            if (row < q.x.rows && col < q.w.rows) {
-                if (q.bias) v += q.bias[col];
-                if (q.act == ANCHA_ACT_GELU) v = gelu_fast(v);
-                if (q.act == ANCHA_ACT_TANH) v = tanh_fast(v);
-                if (q.residual) {
-                    const int64_t at = row * q.ldr + col;
-                    v += q.res_type == ELT_F32    ? static_cast<const float*>(q.residual)[at]
-                         : q.res_type == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(q.residual)[at])
-                                                  : __half2float(static_cast<const __half*>(q.residual)[at]);
-                }
-                if (!mx_out) store_elt(q.out, row * q.ldo + col, v, q.out_type);
-            } else {
-                v = 0.f;
-            }
-            o[ty * 4 + i][tx * 4 + j] = v;
-        }
-    if (!mx_out) return;
-    __syncthreads();
-    // One block of the output's format per thread; scales behind the ends are 0.
-    const int blk = mx_block(om.format), per_row = T / blk;
-    const int64_t okt = mx_ktiles(om.format, om.cols);
-    for (int i = threadIdx.x; i < T * per_row; i += 256) {
-        const int64_t row = m0 + i / per_row;
-        const int c = n0 + i % per_row * blk;
-        if (c / blk >= 4 * okt) continue;
-        const float* v = &o[i / per_row][i % per_row * blk];
-        if (row >= om.rows) om.scales[mx_scale_word(row, c / blk / 4, okt) + c / blk % 4] = 0;
-        else if (om.format == MXF8) quantize_row<MXF8>(om, v, row, c, okt);
-        else if (om.format == MXF4) quantize_row<MXF4>(om, v, row, c, okt);
-        else quantize_row<NVF4>(om, v, row, c, okt);
-    }
+int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
+    if (p.m > 128 && p.n > 128) return launch<FMT, 256, true>(q, p, s);
+    return launch<FMT, 128, false>(q, p, s);
 }
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
 int mx_linear(const MxLinear& q, cudaStream_t s) {
     if (!q.x.rows || !q.w.rows) return ANCHA_OK;
-    // Quantised outputs: whole scale tiles are walked, for the zero scales behind the ends.
-    const MxArray om = q.out_mx ? *q.out_mx : MxArray{};
-    const int64_t m = q.out_mx ? ceil_div(q.x.rows, 128) * 128 : q.x.rows;
-    const int64_t n = q.out_mx ? mx_ktiles(om.format, om.cols) * 4 * mx_block(om.format) : q.w.rows;
-    if (ceil_div(m, T) > 65535) return fail(ANCHA_E_UNSUPPORTED, "mx_linear: too many rows");
-    const dim3 grid((unsigned)ceil_div(n, T), (unsigned)ceil_div(m, T));
-    if (q.x.format == MXF8) linear_kernel<MXF8><<<grid, 256, 0, s>>>(q, om, q.out_mx != nullptr);
-    else if (q.x.format == MXF4) linear_kernel<MXF4><<<grid, 256, 0, s>>>(q, om, q.out_mx != nullptr);
-    else linear_kernel<NVF4><<<grid, 256, 0, s>>>(q, om, q.out_mx != nullptr);
-    return check_launch("mx_linear");
+    Params p{};
+    p.m = (int)q.x.rows; p.n = (int)q.w.rows; p.kbytes = (int)mx_bytes(q.x.format, q.x.cols);
+    p.gx = q.x.global_scale; p.gw = q.w.global_scale;
+    p.bias = q.bias;
+    p.residual = q.residual; p.ldr = q.ldr; p.res_type = q.res_type;
+    p.res_vec = q.residual && aligned16(q.residual) && q.ldr * (int64_t)elt_size(q.res_type) % 16 == 0;
+    p.act = q.act;
+    p.out = q.out; p.ldo = q.ldo; p.out_type = q.out_type;
+    if (q.out_mx) {
+        p.out_mode = OUT_MX;
+        p.om = *q.out_mx;
+        p.okt = (int)mx_ktiles(p.om.format, p.om.cols);
+    } else {
+        p.out_mode = aligned16(q.out) && q.ldo * (int64_t)elt_size(q.out_type) % 16 == 0 ? OUT_TMA : OUT_PLAIN;
+    }
+    p.err = device_error_word();
+    return q.x.format == MXF8 ? by_shape<MXF8>(q, p, s) : q.x.format == MXF4 ? by_shape<MXF4>(q, p, s)
+                                                                             : by_shape<NVF4>(q, p, s);
 }
 
 }  // namespace ancha

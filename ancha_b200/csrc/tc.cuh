@@ -45,6 +45,16 @@ int make_tma_4d(CUtensorMap* map, const void* base, int elt, int64_t cols, int64
 int make_tma_store_3d(CUtensorMap* map, const void* base, int elt, int64_t cols, int64_t rows,
                       int64_t depth, int64_t ld, int64_t depth_stride, int box_cols, int box_rows);
 
+// Encode a tiled tensor map over `rows` rows of `row_bytes` bytes, `ld` bytes apart, with a {box_bytes,
+// box_rows, 1} box; `swizzle`: 128-byte swizzle (box_bytes 128). Zero fill out of bounds.
+int make_tma_bytes(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int64_t ld, int box_bytes,
+                   int box_rows, bool swizzle);
+
+// Encode a tensor map over the scale tiles of a microscaled array (`mt` row ranges of `kt` tiles of 512
+// bytes, as 256-byte rows) with a box of `box_k` tiles along a row by `box_m` row ranges: coordinates
+// {0, 2 · tile, row range}. Zero fill out of bounds.
+int make_tma_scales(CUtensorMap* map, const void* base, int64_t kt, int64_t mt, int box_k, int box_m);
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -148,4 +148,37 @@ int make_tma_4d(CUtensorMap* map, const void* base, int elt, int64_t cols, int64
     return ANCHA_OK;
 }
 
+int make_tma_bytes(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int64_t ld, int box_bytes,
+                   int box_rows, bool swizzle) {
+    auto fn = encode_fn();
+    if (!fn) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+    if (reinterpret_cast<uintptr_t>(base) % 16 || ld % 16 || row_bytes <= 0 || rows <= 0)
+        return fail(ANCHA_E_UNSUPPORTED, "TMA operand not 16-byte aligned");
+    const cuuint64_t dims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)rows, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)ld};
+    const cuuint32_t box[3] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled (bytes) failed: " + std::to_string((int)r));
+    return ANCHA_OK;
+}
+
+int make_tma_scales(CUtensorMap* map, const void* base, int64_t kt, int64_t mt, int box_k, int box_m) {
+    auto fn = encode_fn();
+    if (!fn) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+    if (reinterpret_cast<uintptr_t>(base) % 16 || kt <= 0 || mt <= 0)
+        return fail(ANCHA_E_UNSUPPORTED, "TMA operand not 16-byte aligned");
+    const cuuint64_t dims[3] = {256, (cuuint64_t)(2 * kt), (cuuint64_t)mt};
+    const cuuint64_t strides[2] = {256, (cuuint64_t)(kt * 512)};
+    const cuuint32_t box[3] = {256, (cuuint32_t)(2 * box_k), (cuuint32_t)box_m};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled (scales) failed: " + std::to_string((int)r));
+    return ANCHA_OK;
+}
+
 }  // namespace ancha
