@@ -100,6 +100,8 @@ _lib = None
 def lib() -> C.CDLL:
     """The loaded library (raises AnchaError if it was not built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -110,18 +110,20 @@ __host__ __device__ constexpr uint32_t idesc_of(int m, int n) {
 }
 
 // The products of one slab: `steps` (1 to 4) K steps of 32 bytes. Step i takes scale tile i / (4 / SF) and in
-// it the byte (1X), byte pair (2X) or all four bytes (4X) of its blocks.
+// it the byte (1X), byte pair (2X) or all four bytes (4X) of its blocks. sfa, sfb: TMEM columns of the scales
+// (4 SF, and 4 SF for each 128 columns of the tile or part of them).
 template <int FMT, bool PAIR, int BN>
-__device__ __forceinline__ void slab_products(uint32_t acc, uint32_t tmem, uint32_t a, uint32_t b, uint32_t sa,
+__device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32_t sfb, uint32_t a, uint32_t b, uint32_t sa,
                                               uint32_t sb, uint32_t idesc, int steps, bool first) {
     constexpr int SF = sf_tiles(FMT), PER = 4 / SF;  // K steps per scale tile
+    constexpr int RANGES = BN > 128 ? BN / 128 : 1;  // 128-row ranges of w's scales
 #pragma unroll
     for (int t = 0; t < SF; ++t) {
         if (t * PER >= steps) break;
-        sf_copy<PAIR>(tmem + SFA_COL + 4 * t, sf_desc(sa + t * SF_TILE));
+        sf_copy<PAIR>(sfa + 4 * t, sf_desc(sa + t * SF_TILE));
 #pragma unroll
-        for (int q = 0; q < BN / 128; ++q)
-            sf_copy<PAIR>(tmem + SFB_COL + t * (BN / 32) + 4 * q, sf_desc(sb + (q * SF + t) * SF_TILE));
+        for (int q = 0; q < RANGES; ++q)
+            sf_copy<PAIR>(sfb + 4 * (t * RANGES + q), sf_desc(sb + (q * SF + t) * SF_TILE));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -129,7 +131,7 @@ __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t tmem, uint3
         const int t = i / PER;
         const uint32_t id = FMT == MXF8 ? i : FMT == MXF4 ? i % 2 * 2 : 0;
         mma<FMT, PAIR>(acc, umma_desc_sw128(a + i * 32), umma_desc_sw128(b + i * 32), idesc | id << 4 | id << 29,
-                       tmem + SFA_COL + 4 * t, tmem + SFB_COL + t * (BN / 32), !(first && i == 0));
+                       sfa + 4 * t, sfb + 4 * t * RANGES, !(first && i == 0));
     }
 }
 
@@ -226,6 +228,47 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
     }
     const __half2 t = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// Elements at .. at + nv (at most 4) of a matrix; `vec`: rows and base are 16-byte aligned.
+__device__ __forceinline__ void load4(const void* base, int type, bool vec, int64_t at, int nv, float (&v)[4]) {
+    if (vec && nv == 4) {
+        if (type == ELT_F32) {
+            const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+            return;
+        }
+        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
+        const uint32_t u[2] = {q.x, q.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 f = type == ELT_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]))
+                                              : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < nv)
+            v[j] = type == ELT_F32    ? static_cast<const float*>(base)[at + j]
+                   : type == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at + j])
+                                      : __half2float(static_cast<const __half*>(base)[at + j]);
+}
+
+__device__ __forceinline__ void store4(void* base, int type, bool vec, int64_t at, int nv, const float (&v)[4]) {
+    if (vec && nv == 4) {
+        if (type == ELT_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
+                make_uint2(pack16(v[0], v[1], type), pack16(v[2], v[3], type));
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < nv) store_elt(base, at + j, v[j], type);
 }
 
 // A lane's row of 32 values in the swizzled staging layout of the TMA store (128-byte rows of f32 with the
@@ -408,7 +451,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     if (!mbar_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
                     tc_fence_after();
                     const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
-                    slab_products<FMT, PAIR, BN>(acc, tmem, smem_u32(a_tiles + s * OPERAND_BYTES),
+                    slab_products<FMT, PAIR, BN>(acc, tmem + SFA_COL, tmem + SFB_COL, smem_u32(a_tiles + s * OPERAND_BYTES),
                                                  smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
                                                  smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0);
                     if (PAIR) umma_commit_pair(&empty[s], 0x3);
@@ -497,6 +540,242 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     }
 }
 
+// ---- few tiles ------------------------------------------------------------------------------
+
+// Few rows of x, or few tiles: a cluster of `splits` CTAs shares one tile, each multiplying a part of K, so that
+// the weight streams through many SMs. The operands change places: 128 rows of w are the instruction's M and TN rows
+// of x its N, so a single token costs 16 columns instead of 128 rows. Each CTA leaves its partial sums in its
+// shared memory (over the operands, which are done with); then rank r of the cluster finishes the rows r, r + splits,
+// ... of x, adding the ranks' sums in rank order through distributed shared memory. A warp takes a row of x and the
+// tile's 128 columns, four to a lane.
+template <int FMT, int TN>
+struct SplitShape {
+    static constexpr int SF = sf_tiles(FMT);
+    static constexpr int STAGE = OPERAND_BYTES + TN * SLAB + 2 * SF * SF_TILE;
+    static constexpr int FIT = (113 * 1024 - 1280) / STAGE, STAGES = FIT < 5 ? FIT : 5;  // two CTAs per SM
+    static constexpr int BYTES = 1024 + STAGES * STAGE + 256;
+    static constexpr uint32_t COLS = TN == 128 ? 256 : TN == 64 ? 128 : 64;
+    static_assert(TN + 8 * SF <= (int)COLS, "accumulator and scales do not fit");
+    static_assert(TN * BM * 4 <= STAGES * STAGE && BYTES <= 113 * 1024, "shared memory");
+};
+constexpr int SPLIT_WARPS = 6, SPLIT_THREADS = 32 * SPLIT_WARPS;
+
+// Four neighbouring columns per lane, a warp's 128 from c0 on (zeros behind the row's end), quantised.
+template <int FMT>
+__device__ __forceinline__ void store_mx_lanes(const MxArray& o, int okt, int64_t row, int c0, int lane, const float (&v)[4]) {
+    constexpr int B = mx_block(FMT), LB = B / 4;  // lanes of a block
+    const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
+    uint32_t a = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+#pragma unroll
+    for (int d = 1; d < LB; d *= 2) a = max(a, __shfl_xor_sync(0xffffffffu, a, d));
+    const MxBlock b = mx_block_scale<FMT>(a, g);
+    const uint32_t lo = mx_pair<FMT>(mx_scaled<FMT>(v[0], b), mx_scaled<FMT>(v[1], b));
+    const uint32_t hi = mx_pair<FMT>(mx_scaled<FMT>(v[2], b), mx_scaled<FMT>(v[3], b));
+    const int c = c0 + 4 * lane;
+    if (mx_bytes(FMT, c) < mx_row_bytes(FMT, o.cols)) {
+        uint8_t* d = o.data + row * o.ld + mx_bytes(FMT, c);
+        if (FMT == MXF8) *reinterpret_cast<uint32_t*>(d) = lo | hi << 16;
+        else *reinterpret_cast<uint16_t*>(d) = (uint16_t)(lo | hi << 8);
+    }
+    if (lane % LB == 0 && c / B < 4 * okt) o.scales[mx_scale_word(row, c / B / 4, okt) + c / B % 4] = (uint8_t)b.code;
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+template <int FMT, int TN>
+__global__ void __launch_bounds__(SPLIT_THREADS)
+split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+             const __grid_constant__ CUtensorMap tsw, const __grid_constant__ CUtensorMap tsx,
+             const __grid_constant__ Params p, int splits) {
+    using S = SplitShape<FMT, TN>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* w_tiles = smem;
+    uint8_t* x_tiles = w_tiles + STAGES * OPERAND_BYTES;
+    uint8_t* sw_tiles = x_tiles + STAGES * TN * SLAB;
+    uint8_t* sx_tiles = sw_tiles + STAGES * S::SF * SF_TILE;
+    float* partial = reinterpret_cast<float*>(smem);  // [TN][128], once the products are done
+    uint64_t* full = reinterpret_cast<uint64_t*>(sx_tiles + STAGES * S::SF * SF_TILE);
+    uint64_t* empty = full + STAGES;
+    uint64_t* done = empty + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = (int)blockIdx.x % splits, n0 = (int)blockIdx.x / splits * BM, m0 = (int)blockIdx.y * TN;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        *abort = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+        prefetch_tma(&tw);
+        prefetch_tma(&tx);
+        prefetch_tma(&tsw);
+        prefetch_tma(&tsx);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, S::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int slabs = (p.kbytes + SLAB - 1) / SLAB;
+    const int kb0 = (int)((int64_t)slabs * rank / splits), kb1 = (int)((int64_t)slabs * (rank + 1) / splits);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+                mbar_arrive_expect_tx(&full[s], S::STAGE);
+                tma_load_3d(w_tiles + s * OPERAND_BYTES, &tw, &full[s], kb * SLAB, n0, 0);
+                tma_load_3d(sw_tiles + s * S::SF * SF_TILE, &tsw, &full[s], 0, kb * S::SF * 2, n0 / 128);
+                tma_load_3d(x_tiles + s * TN * SLAB, &tx, &full[s], kb * SLAB, m0, 0);
+                tma_load_3d(sx_tiles + s * S::SF * SF_TILE, &tsx, &full[s], 0, kb * S::SF * 2, m0 / 128);
+            }
+            if (*abort) {  // let copies in flight land before the CTA exits (bounded)
+                const long long c0 = clock64();
+                for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
+                    while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
+                    }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_of<FMT>(BM, TN);
+            uint32_t it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!mbar_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
+                tc_fence_after();
+                const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
+                slab_products<FMT, false, TN>(tmem, tmem + TN, tmem + TN + 4 * S::SF, smem_u32(w_tiles + s * OPERAND_BYTES),
+                                              smem_u32(x_tiles + s * TN * SLAB), smem_u32(sw_tiles + s * S::SF * SF_TILE),
+                                              smem_u32(sx_tiles + s * S::SF * SF_TILE), idesc, steps, kb == kb0);
+                umma_commit(&empty[s]);
+            }
+            umma_commit(done);
+        }
+        __syncwarp();
+    }
+    const int live = min(TN, p.m - m0);  // rows of x in the tile
+    if (warp >= 2) {
+        const int quarter = warp % 4;
+        if (__all_sync(0xffffffffu, mbar_wait(done, 0, abort, p.err))) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < live; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + c + ((uint32_t)(quarter * 32) << 16), r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) partial[(c + j) * BM + quarter * 32 + lane] = __uint_as_float(r[j]);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::COLS);
+    }
+    float alpha = 1.f;
+    if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
+    const int col = n0 + 4 * lane, nv = min(4, p.n - col);  // this lane's columns
+    float bias[4] = {};
+    if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < nv) bias[j] = p.bias[col + j];
+    }
+    for (int c = rank + warp * splits; c < live; c += SPLIT_WARPS * splits) {
+        const int64_t row = m0 + c;
+        float res[4] = {};
+        if (p.residual) load4(p.residual, p.res_type, p.res_vec, row * p.ldr + col, nv, res);
+        float v[4] = {};
+        const uint32_t at = smem_u32(partial + c * BM + 4 * lane);
+        for (int k = 0; k < splits; ++k) {
+            const float4 q = ld_cluster4(mapa_shared(at, k));
+            v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(v[j], alpha, bias[j]);
+        if (p.act == ANCHA_ACT_GELU) {
+            gelu2(v[0], v[1]);
+            gelu2(v[2], v[3]);
+        } else if (p.act == ANCHA_ACT_TANH) {
+            tanh_fast2(v[0], v[1]);
+            tanh_fast2(v[2], v[3]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = j < nv ? v[j] + res[j] : 0.f;
+        if (p.out_mode != OUT_MX) store4(p.out, p.out_type, p.out_mode == OUT_TMA, row * p.ldo + col, nv, v);
+        else if (p.om.format == MXF8) store_mx_lanes<MXF8>(p.om, p.okt, row, n0, lane, v);
+        else if (p.om.format == MXF4) store_mx_lanes<MXF4>(p.om, p.okt, row, n0, lane, v);
+        else store_mx_lanes<NVF4>(p.om, p.okt, row, n0, lane, v);
+    }
+    // Quantised output: the scales of the rows behind the last, in its tile, are 0 (the last row tile's CTAs share them).
+    if (p.out_mode == OUT_MX && blockIdx.y == gridDim.y - 1) {
+        const int b = mx_block(p.om.format);
+        const int64_t end = ((int64_t)p.m + 127) / 128 * 128;
+        const int words = max(0, min(p.okt - n0 / (4 * b), BM / (4 * b)));
+        for (int64_t i = rank * SPLIT_THREADS + threadIdx.x; i < (end - p.m) * words; i += splits * SPLIT_THREADS)
+            *reinterpret_cast<uint32_t*>(p.om.scales + mx_scale_word(p.m + i / words, n0 / (4 * b) + (int)(i % words), p.okt)) = 0;
+    }
+    __syncwarp();
+    cluster_sync();  // a CTA's shared memory stays while its peers read it
+}
+
+template <int FMT, int TN>
+int launch_split(const MxLinear& q, const Params& p, int splits, cudaStream_t s) {
+    using S = SplitShape<FMT, TN>;
+    auto kernel = split_kernel<FMT, TN>;
+    static bool configured[64] = {};
+    int dev = 0;
+    ANCHA_CUDA(cudaGetDevice(&dev));
+    if (!configured[dev & 63]) {
+        ANCHA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+        configured[dev & 63] = true;
+    }
+    CUtensorMap tw, tx, tsw, tsx;
+    const int64_t kt = mx_ktiles(FMT, q.x.cols);
+    ANCHA_TRY(make_tma_bytes(&tw, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, BM, true));
+    ANCHA_TRY(make_tma_bytes(&tx, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, TN, true));
+    ANCHA_TRY(make_tma_scales(&tsw, q.w.scales, kt, ceil_div(p.n, 128), S::SF, 1));
+    ANCHA_TRY(make_tma_scales(&tsx, q.x.scales, kt, ceil_div(p.m, 128), S::SF, 1));
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ceil_div(p.n, BM) * splits), (unsigned)ceil_div(p.m, TN), 1);
+    cfg.blockDim = dim3(SPLIT_THREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::BYTES;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ANCHA_CUDA(cudaLaunchKernelEx(&cfg, kernel, tw, tx, tsw, tsx, p, splits));
+    return check_launch("mx_linear (split)");
+}
+
 template <int FMT, int BN, bool PAIR>
 int launch(const MxLinear& q, Params p, cudaStream_t s) {
     using S = Shape<FMT, BN, PAIR>;
@@ -549,6 +828,15 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
 
 template <int FMT>
 int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
+    const int64_t row_tiles = p.m <= 64 ? 1 : ceil_div(p.m, 128), tiles = row_tiles * ceil_div(p.n, 128);
+    if (p.m <= 64 || tiles <= 74) {
+        const int slabs = (int)ceil_div(p.kbytes, SLAB);
+        int splits = 1;
+        while (splits < 8 && 2 * splits <= slabs && tiles * 2 * splits <= 296) splits *= 2;
+        if (p.m <= 16) return launch_split<FMT, 16>(q, p, splits, s);
+        if (p.m <= 64) return launch_split<FMT, 64>(q, p, splits, s);
+        return launch_split<FMT, 128>(q, p, splits, s);
+    }
     if (p.m > 128 && p.n > 128) return launch<FMT, 256, true>(q, p, s);
     return launch<FMT, 128, false>(q, p, s);
 }

@@ -21,8 +21,8 @@ They raise ``AnchaError`` for arguments they do not take. No gradients: this is 
 """
 from __future__ import annotations
 
-import ctypes as C
-from dataclasses import dataclass
+import functools
+from ctypes import byref
 from typing import Optional
 
 import torch
@@ -35,18 +35,61 @@ ACTIVATIONS = {"none": N.ACT_NONE, "gelu": N.ACT_GELU, "tanh": N.ACT_TANH}
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 
 
-@dataclass(frozen=True)
+def _invalid(message: str) -> N.AnchaError:
+    return N.AnchaError(N.E_INVALID, message)
+
+
+@functools.lru_cache(maxsize=256)
+def _layout(fmt: str, rows: int, cols: int):
+    """(bytes from row to row, shape of the scales, bytes of the elements, bytes of the scales):
+    ``ancha_mx_layout``'s rule."""
+    if fmt not in FORMATS:
+        raise _invalid(f"unknown format {fmt!r}: one of {', '.join(FORMATS)}")
+    if cols < 1 or rows < 0:
+        raise _invalid("rows without elements, or a negative number of rows")
+    ld = -(-(cols if fmt == "mxf8" else (cols + 1) // 2) // 16) * 16
+    mt, kt = -(-rows // 128), -(-cols // (4 * BLOCK[fmt]))
+    return ld, (mt, kt, 32, 4, 4), rows * ld, mt * kt * 512
+
+
 class Microscaled:
-    """Rows of quantised elements. ``data``: uint8 ``[rows, ld]``, elements in memory order (two per byte
-    in the 4-bit formats, the even column in the low half). ``scales``: uint8 ``[rows / 128, blocks / 4,
-    32, 4, 4]`` (both rounded up): the code of (row, block) at ``[row // 128, block // 4, row % 32,
-    row % 128 // 32, block % 4]``. ``global_scale``: one f32 on the device (``nvf4`` only; None is 1)."""
-    format: str
-    rows: int
-    cols: int
-    data: torch.Tensor
-    scales: torch.Tensor
-    global_scale: Optional[torch.Tensor] = None
+    """Rows of quantised elements.
+
+    ``data``: uint8 ``[rows, ld]``, elements in memory order (two per byte in the 4-bit formats, the even
+    column in the low half), ``ld`` a multiple of 16. ``scales``: uint8 ``[rows / 128, blocks / 4, 32, 4, 4]``
+    (both rounded up): the code of (row, block) at ``[row // 128, block // 4, row % 32, row % 128 // 32,
+    block % 4]``. ``global_scale``: one f32 on the device (``nvf4`` only; None is 1).
+    """
+    __slots__ = ("format", "rows", "cols", "global_scale", "_data", "_scales", "_buffer")
+
+    def __init__(self, format: str, rows: int, cols: int, data: torch.Tensor, scales: torch.Tensor,
+                 global_scale: Optional[torch.Tensor] = None):
+        self.format, self.rows, self.cols, self.global_scale = format, rows, cols, global_scale
+        self._data, self._scales, self._buffer = data, scales, None
+
+    @classmethod
+    def _new(cls, format, rows, cols, like, global_scale):
+        """An array in one new allocation on the device of ``like``: elements, then scales."""
+        q = object.__new__(cls)
+        q.format, q.rows, q.cols, q.global_scale = format, rows, cols, global_scale
+        _, _, data, scales = _layout(format, rows, cols)
+        q._buffer = like.new_empty(data + scales, dtype=torch.uint8)
+        q._data = q._scales = None
+        return q
+
+    @property
+    def data(self) -> torch.Tensor:
+        if self._data is None:
+            ld = _layout(self.format, self.rows, self.cols)[0]
+            self._data = self._buffer.as_strided((self.rows, ld), (ld, 1), 0)
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            _, shape, offset, _ = _layout(self.format, self.rows, self.cols)
+            self._scales = self._buffer.as_strided(shape, (shape[1] * 512, 512, 16, 4, 1), offset)
+        return self._scales
 
     def scale_codes(self) -> torch.Tensor:
         """The scale codes as a uint8 ``[rows, blocks]`` matrix (a copy)."""
@@ -55,100 +98,100 @@ class Microscaled:
         return s.permute(0, 3, 2, 1, 4).reshape(s.shape[0] * 128, -1)[:self.rows, :blocks]
 
 
-def _invalid(message: str) -> N.AnchaError:
-    return N.AnchaError(N.E_INVALID, message)
-
-
-def _shapes(fmt: str, rows: int, cols: int):
-    """Shapes of ``data`` and ``scales`` (``ancha_mx_layout``'s rule)."""
-    if fmt not in FORMATS:
-        raise _invalid(f"unknown format {fmt!r}: one of {', '.join(FORMATS)}")
-    if cols < 1:
-        raise _invalid("rows without elements")
-    ld = -(-(cols if fmt == "mxf8" else (cols + 1) // 2) // 16) * 16
-    return (rows, ld), (-(-rows // 128), -(-cols // (4 * BLOCK[fmt])), 32, 4, 4)
-
-
 def empty(format: str, rows: int, cols: int, device="cuda", global_scale=None) -> Microscaled:
     """An array with memory for ``rows`` by ``cols`` elements, not yet written."""
-    data, scales = _shapes(format, rows, cols)
-    return Microscaled(format, rows, cols, torch.empty(data, dtype=torch.uint8, device=device),
-                       torch.empty(scales, dtype=torch.uint8, device=device), global_scale)
+    return Microscaled._new(format, rows, cols, torch.empty(0, device=device), global_scale)
 
 
-class _Call:
-    """The device and stream of a call, and the check that its tensors live there."""
+def _device(t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise _invalid("tensors must be on a CUDA device")
+    return t.get_device()
 
-    def __init__(self, tensor):
-        if not tensor.is_cuda:
-            raise _invalid("tensors must be on a CUDA device")
-        self.index = tensor.device.index
 
-    def on(self, t, name: str):
-        if not t.is_cuda or t.device.index != self.index:
-            raise _invalid(f"{name}: not on the device of the first operand")
-        return t
+def _on(t, device: int, name: str):
+    if t.get_device() != device:
+        raise _invalid(f"{name}: not on the device of the first operand")
 
-    def vector(self, t, name: str, n: int):
-        """Address of a contiguous f32 vector of n elements, None for None."""
-        if t is None:
-            return None
-        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
-            raise _invalid(f"{name}: needs {n} contiguous f32 elements")
-        return self.on(t, name).data_ptr()
 
-    def matrix(self, t, name: str):
-        """(dtype code, row stride) of a 2-D tensor whose rows are dense."""
-        code = _DTYPES.get(t.dtype)
-        if code is None:
-            raise _invalid(f"{name}: unsupported dtype {t.dtype}")
-        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-            raise _invalid(f"{name}: needs two axes, the last one contiguous")
-        self.on(t, name)
-        # The stride of a single row is arbitrary in torch.
-        return code, (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+def _vector(t, device: int, n: int, name: str):
+    """Address of a contiguous f32 vector of n elements, None for None."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise _invalid(f"{name}: needs {n} contiguous f32 elements")
+    _on(t, device, name)
+    return t.data_ptr()
 
-    def array(self, q: Microscaled, name: str) -> N.MxArray:
-        data, scales = _shapes(q.format, q.rows, q.cols)
-        if q.data.dtype != torch.uint8 or q.data.dim() != 2 or q.data.shape[0] != q.rows \
-                or q.data.shape[1] < data[1] or q.data.stride(1) != 1:
-            raise _invalid(f"{name}: data is not uint8 [rows, >= {data[1]}] with contiguous rows")
-        if q.scales.dtype != torch.uint8 or tuple(q.scales.shape) != scales or not q.scales.is_contiguous():
-            raise _invalid(f"{name}: scales are not contiguous uint8 {scales}")
-        self.on(q.data, name)
-        self.on(q.scales, name)
-        ld = q.data.stride(0) if q.rows > 1 else data[1]
-        return N.MxArray(FORMATS[q.format], q.rows, q.cols, q.data.data_ptr(), ld, q.scales.data_ptr(),
-                         self.vector(q.global_scale, f"{name}: global_scale", 1))
 
-    def run(self, fn, *args):
-        """Call the library with torch's current stream of the tensors' device, which is made current."""
-        if torch.cuda.current_device() == self.index:
-            N.check(fn(*args, torch.cuda.current_stream(self.index).cuda_stream))
-        else:
-            with torch.cuda.device(self.index):
-                N.check(fn(*args, torch.cuda.current_stream(self.index).cuda_stream))
+def _matrix(t, device: int, name: str):
+    """(dtype code, row stride) of a 2-D tensor whose rows are dense."""
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise _invalid(f"{name}: unsupported dtype {t.dtype}")
+    if t.dim() != 2:
+        raise _invalid(f"{name}: needs two axes")
+    _on(t, device, name)
+    rows, cols = t.shape
+    if rows <= 1 and cols <= 1 or t.is_contiguous():  # the stride of a single row is arbitrary in torch
+        return code, max(cols, 1)
+    if cols > 1 and t.stride(1) != 1:
+        raise _invalid(f"{name}: its last axis must be contiguous")
+    return code, (t.stride(0) if rows > 1 else cols)
+
+
+def _array(q: Microscaled, device: int, name: str) -> N.MxArray:
+    ld, shape, data_bytes, _ = _layout(q.format, q.rows, q.cols)
+    g = None if q.global_scale is None else _vector(q.global_scale, device, 1, f"{name}: global_scale")
+    buffer = q._buffer
+    if buffer is not None:
+        _on(buffer, device, name)
+        at = buffer.data_ptr()
+        return N.MxArray(FORMATS[q.format], q.rows, q.cols, at, ld, at + data_bytes, g)
+    data, scales = q._data, q._scales
+    if data.dtype != torch.uint8 or data.dim() != 2 or data.shape[0] != q.rows or data.shape[1] < ld \
+            or data.stride(1) != 1:
+        raise _invalid(f"{name}: data is not uint8 [{q.rows}, >= {ld}] with contiguous rows")
+    if scales.dtype != torch.uint8 or scales.shape != shape or not scales.is_contiguous():
+        raise _invalid(f"{name}: scales are not contiguous uint8 {shape}")
+    _on(data, device, name)
+    _on(scales, device, name)
+    return N.MxArray(FORMATS[q.format], q.rows, q.cols, data.data_ptr(), data.stride(0) if q.rows > 1 else ld,
+                     scales.data_ptr(), g)
+
+
+def _run(device: int, fn, *args):
+    """Call the library on torch's current stream of `device`, which is made current for the call."""
+    if torch._C._cuda_getDevice() == device:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        N.check(status)
 
 
 def quantize(x: torch.Tensor, format: str = "mxf8", global_scale: Optional[torch.Tensor] = None) -> Microscaled:
     """Quantise the rows of ``x [rows, cols]`` (f32, bf16 or f16; any row stride). Scales and rounding as
     ``ancha_mx_quantize`` says. ``global_scale`` (``nvf4``): one f32 on the device, usually
     ``max|x| / (6 * 448)``; it becomes the array's."""
-    call = _Call(x)
-    dtype, ld = call.matrix(x, "x")
-    out = empty(format, x.shape[0], x.shape[1], x.device, global_scale)
-    call.run(N.lib().ancha_mx_quantize, x.data_ptr(), dtype, ld, C.byref(call.array(out, "out")))
+    device = _device(x)
+    dtype, ld = _matrix(x, device, "x")
+    rows, cols = x.shape
+    out = Microscaled._new(format, rows, cols, x, global_scale)
+    _run(device, N.lib().ancha_mx_quantize, x.data_ptr(), dtype, ld, byref(_array(out, device, "out")))
     return out
 
 
 def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``q`` stands for, ``[rows, cols]`` in ``dtype`` (f32, bf16 or f16)."""
-    call = _Call(q.data)
+    device = _device(q._data if q._buffer is None else q._buffer)
     code = _DTYPES.get(dtype)
     if code is None:
         raise _invalid(f"unsupported dtype {dtype}")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.data.device)
-    call.run(N.lib().ancha_mx_dequantize, C.byref(call.array(q, "q")), out.data_ptr(), code, q.cols)
+    a = _array(q, device, "q")
+    out = torch.empty((q.rows, q.cols), dtype=dtype, device=(q._data if q._buffer is None else q._buffer).device)
+    _run(device, N.lib().ancha_mx_dequantize, byref(a), out.data_ptr(), code, q.cols)
     return out
 
 
@@ -159,26 +202,27 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, gain:
     ``s / sqrt(mean(s^2) + eps) * gain``. Returns ``(Microscaled, s)``; ``s`` has the residual's dtype and
     is ``x`` itself without a residual. ``residual_out`` takes ``s`` (``residual`` itself: in place).
     ``x`` and ``residual``: f32, bf16 or f16 ``[rows, cols]``, at most 32768 columns; ``gain``: f32 ``[cols]``."""
-    call = _Call(x)
-    dtype, ldx = call.matrix(x, "x")
+    device = _device(x)
+    dtype, ldx = _matrix(x, device, "x")
     rows, cols = x.shape
-    res_type, ldr, ldro = dtype, ldx, ldx
+    stream, res_type, ldr, ldro, res, res_out = x, dtype, ldx, ldx, None, None
     if residual is not None:
         if residual.shape != x.shape:
             raise _invalid("residual: not the shape of x")
-        res_type, ldr = call.matrix(residual, "residual")
+        res_type, ldr = _matrix(residual, device, "residual")
+        res = residual.data_ptr()
         if residual_out is None:
             residual_out = torch.empty((rows, cols), dtype=residual.dtype, device=x.device)
-    if residual_out is not None:
+            stream, ldro, res_out = residual_out, cols, residual_out.data_ptr()
+    if residual_out is not None and stream is x:
         if residual_out.shape != x.shape or residual_out.dtype != (x if residual is None else residual).dtype:
             raise _invalid("residual_out: not the shape and dtype of the residual stream")
-        ldro = call.matrix(residual_out, "residual_out")[1]
-    out = empty(format, rows, cols, x.device, global_scale)
-    desc = N.MxNormDesc(dtype, res_type, ldx, ldr, ldro, eps)
-    call.run(N.lib().ancha_mx_add_rms_norm_fwd, C.byref(desc), x.data_ptr(),
-             None if residual is None else residual.data_ptr(), call.vector(gain, "gain", cols),
-             None if residual_out is None else residual_out.data_ptr(), C.byref(call.array(out, "out")))
-    return out, (x if residual_out is None else residual_out)
+        ldro = _matrix(residual_out, device, "residual_out")[1]
+        stream, res_out = residual_out, residual_out.data_ptr()
+    out = Microscaled._new(format, rows, cols, x, global_scale)
+    _run(device, N.lib().ancha_mx_add_rms_norm_fwd, byref(N.MxNormDesc(dtype, res_type, ldx, ldr, ldro, eps)), x.data_ptr(),
+         res, _vector(gain, device, cols, "gain"), res_out, byref(_array(out, device, "out")))
+    return out, stream
 
 
 def linear(x: Microscaled, weight: Microscaled, bias: Optional[torch.Tensor] = None, act: str = "none",
@@ -188,24 +232,24 @@ def linear(x: Microscaled, weight: Microscaled, bias: Optional[torch.Tensor] = N
     f32 accumulation. ``act``: ``"none"``, ``"gelu"`` (erf) or ``"tanh"``; ``bias`` f32; ``residual`` f32, bf16
     or f16. The result is a tensor of ``dtype`` (default bf16), or with ``format`` a quantised array
     (``global_scale`` as in :func:`quantize`)."""
-    call = _Call(x.data)
+    memory = x._data if x._buffer is None else x._buffer
+    device = _device(memory)
     if act not in ACTIVATIONS:
         raise _invalid(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
-    if dtype is not None and format is not None:
-        raise _invalid("dtype and format exclude each other")
     m, n = x.rows, weight.rows
-    res_type, ldr = N.F32, 0
+    res, res_type, ldr = None, N.F32, 0
     if residual is not None:
-        if tuple(residual.shape) != (m, n):
+        if residual.shape != (m, n):
             raise _invalid("residual: not the shape of the product")
-        res_type, ldr = call.matrix(residual, "residual")
-    a, w, b = call.array(x, "x"), call.array(weight, "weight"), call.vector(bias, "bias", n)
-    res = None if residual is None else residual.data_ptr()
+        res_type, ldr = _matrix(residual, device, "residual")
+        res = residual.data_ptr()
+    a, w, b = _array(x, device, "x"), _array(weight, device, "weight"), _vector(bias, device, n, "bias")
     if format is not None:
-        out = empty(format, m, n, x.data.device, global_scale)
-        desc = N.MxLinearDesc(ACTIVATIONS[act], N.F32, res_type, n, ldr)
-        call.run(N.lib().ancha_mx_linear_fwd, C.byref(desc), C.byref(a), C.byref(w), b, res, None,
-                 C.byref(call.array(out, "out")))
+        if dtype is not None:
+            raise _invalid("dtype and format exclude each other")
+        out = Microscaled._new(format, m, n, memory, global_scale)
+        _run(device, N.lib().ancha_mx_linear_fwd, byref(N.MxLinearDesc(ACTIVATIONS[act], N.F32, res_type, n, ldr)), byref(a),
+             byref(w), b, res, None, byref(_array(out, device, "out")))
         return out
     if global_scale is not None:
         raise _invalid("global_scale without format")
@@ -213,7 +257,7 @@ def linear(x: Microscaled, weight: Microscaled, bias: Optional[torch.Tensor] = N
     code = _DTYPES.get(dtype)
     if code is None:
         raise _invalid(f"unsupported dtype {dtype}")
-    out = torch.empty((m, n), dtype=dtype, device=x.data.device)
-    desc = N.MxLinearDesc(ACTIVATIONS[act], code, res_type, n, ldr)
-    call.run(N.lib().ancha_mx_linear_fwd, C.byref(desc), C.byref(a), C.byref(w), b, res, out.data_ptr(), None)
+    out = torch.empty((m, n), dtype=dtype, device=memory.device)
+    _run(device, N.lib().ancha_mx_linear_fwd, byref(N.MxLinearDesc(ACTIVATIONS[act], code, res_type, n, ldr)), byref(a),
+         byref(w), b, res, out.data_ptr(), None)
     return out

@@ -9,6 +9,7 @@ of |y|. Products: operands and their products are exact in f32, so the sum of k 
 step. A quantised result is off by half a step of its elements more, and its scale is that of a maximum within
 the tolerance."""
 import math
+from ctypes import byref
 
 import numpy as np
 import pytest
@@ -189,8 +190,7 @@ def test_strides_offsets_and_memory_behind_the_array(fmt):
     wide = torch.full((40, 512), 0xAB, dtype=torch.uint8, device="cuda")
     q = mx.empty(fmt, rows, cols)
     q = mx.Microscaled(fmt, rows, cols, wide[:rows], q.scales)
-    call = mx._Call(x)
-    N.check(N.lib().ancha_mx_quantize(x.data_ptr(), N.BF16, 700, mx.C.byref(call.array(q, "q")), 0))
+    N.check(N.lib().ancha_mx_quantize(x.data_ptr(), N.BF16, 700, byref(mx._array(q, 0, "q")), 0))
     width = -(-(cols if fmt == "mxf8" else (cols + 1) // 2) // 16) * 16
     assert (wide[rows:] == 0xAB).all() and (wide[:, width:] == 0xAB).all()
     check_exact(mx.Microscaled(fmt, rows, cols, wide[:rows, :width].contiguous(), q.scales), f64(x))
@@ -398,8 +398,7 @@ def test_linear_strides_and_offsets(fmt, m, n):
         ref = buf.clone()
         ref[1:m + 1, lo:lo + n] = want
         d = N.MxLinearDesc(N.ACT_GELU, N.BF16, N.BF16, ld + 8, ld + 8)
-        call = mx._Call(x.data)
-        N.check(N.lib().ancha_mx_linear_fwd(mx.C.byref(d), mx.C.byref(call.array(x, "x")), mx.C.byref(call.array(w, "w")),
+        N.check(N.lib().ancha_mx_linear_fwd(byref(d), byref(mx._array(x, 0, "x")), byref(mx._array(w, 0, "w")),
                                             bias.data_ptr(), view.data_ptr(), view.data_ptr(), None, 0))
         assert torch.equal(buf, ref)
 
