@@ -133,26 +133,79 @@ __device__ __forceinline__ MxBlock mx_block_scale(uint32_t amax_bits, float glob
     return b;
 }
 
-template <int FMT>
-__device__ __forceinline__ float mx_scaled(float v, const MxBlock& b) {
-    if (!b.live) return 0.f;
-    return FMT == NVF4 ? __fdiv_rn(v, b.factor) : v * b.factor;
+// max(m, |a|, |b|); NaN where one is.
+__device__ __forceinline__ float absmax(float m, float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
 }
 
-// Two elements: E4M3 codes in the two bytes of the result, or E2M1 codes in the two halves of one byte.
-template <int FMT>
-__device__ __forceinline__ uint32_t mx_pair(float lo, float hi) {
-    if (FMT == MXF8) return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-    return __nv_cvt_float2_to_fp4x2(make_float2(lo, hi), __NV_E2M1, cudaRoundNearest);
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
 }
+__device__ __forceinline__ uint32_t pack_e2m1(const float (&v)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+
+// Codes of N elements of one block (or a part of one), 4 or 8 to a word.
+// NVF4: dividing every element costs eight instructions or more. The product with the rounded reciprocal is off
+// by less than 2^-22 of the quotient, so where rounding it down and up by 2^-21 gives one code that is the
+// quotient's too; otherwise (next to a border) the elements are divided.
+template <int FMT, int N>
+__device__ __forceinline__ void mx_encode(const float (&v)[N], const MxBlock& b, uint32_t (&w)[N / (FMT == MXF8 ? 4 : 8)]) {
+    constexpr int PER = FMT == MXF8 ? 4 : 8, W = N / PER;
+    const uint32_t mask = b.live ? 0xffffffffu : 0u;
+    if constexpr (FMT == NVF4) {
+        const float r = __frcp_rn(b.factor), lo = r * (1.f - 0x1p-21f), hi = r * (1.f + 0x1p-21f);
+        bool same = b.factor > 1e-30f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float t[8], u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                t[j] = v[8 * i + j] * lo;
+                u[j] = v[8 * i + j] * hi;
+            }
+            w[i] = pack_e2m1(t) & mask;
+            same = same && w[i] == (pack_e2m1(u) & mask);
+        }
+        if (!same && b.live) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                float t[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = __fdiv_rn(v[8 * i + j], b.factor);
+                w[i] = pack_e2m1(t);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            float t[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) t[j] = v[PER * i + j] * b.factor;
+            if constexpr (FMT == MXF8) w[i] = pack_e4m3(t[0], t[1], t[2], t[3]) & mask;
+            else w[i] = pack_e2m1(t) & mask;
+        }
+    }
+}
+
 template <int FMT>
 __device__ __forceinline__ float2 mx_pair_values(uint32_t code) {
     const __half2_raw h = FMT == MXF8 ? __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code, __NV_E4M3)
                                       : __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)code, __NV_E2M1);
     return __half22float2(__half2(h));
 }
-
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 #endif  // __CUDACC__
 

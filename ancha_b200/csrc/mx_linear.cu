@@ -22,7 +22,7 @@ namespace {
 constexpr int BM = 128, SLAB = 128;          // rows of a CTA's tile, bytes of a K slab
 constexpr int OPERAND_BYTES = BM * SLAB;     // 128 rows of a slab
 constexpr int SF_TILE = 512;                 // a scale tile
-constexpr int EPI = 8;                       // epilogue warps
+constexpr int EPI = 16;                      // epilogue warps
 constexpr int THREADS = 64 + 32 * EPI;
 constexpr int STAGING = 4096;                // per epilogue warp: 32 rows x 128 bytes
 // TMEM: two accumulators, then the scales of the slab in work.
@@ -54,7 +54,7 @@ struct Params {
     const float* bias;
     const void* residual;
     int64_t ldr;
-    int res_type, res_vec, act;
+    int res_type, res_vec, bias_vec, act;
     void* out;
     int64_t ldo;
     int out_type, out_mode;    // OUT_*
@@ -161,22 +161,26 @@ __device__ __forceinline__ float residual_at(const Params& p, int64_t i) {
                                     : __half2float(static_cast<const __half*>(p.residual)[i]);
 }
 
-// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them).
+// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them). The arithmetic
+// runs on packed pairs, one instruction for two values: the epilogue is bound by instruction issue.
+template <bool SCALED>
 __device__ __forceinline__ void finish32(const Params& p, int64_t row, bool live, int c0, int nv, float alpha,
                                          const uint32_t (&r)[32], float (&v)[32]) {
+    const uint64_t al = f2(alpha, alpha);
+    if (p.bias && p.bias_vec && nv == 32) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * alpha;
-    if (p.bias) {
-        if (nv == 32 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0) {
+        for (int j = 0; j < 32; j += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p.bias + c0 + j);
+            const uint64_t a = f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+            const uint64_t b = f2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+            f2_split(SCALED ? ffma2(a, al, f2(q.x, q.y)) : fadd2(a, f2(q.x, q.y)), v[j], v[j + 1]);
+            f2_split(SCALED ? ffma2(b, al, f2(q.z, q.w)) : fadd2(b, f2(q.z, q.w)), v[j + 2], v[j + 3]);
+        }
+    } else {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(p.bias + c0 + j);
-                v[j] += q.x; v[j + 1] += q.y; v[j + 2] += q.z; v[j + 3] += q.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < nv) v[j] += p.bias[c0 + j];
+        for (int j = 0; j < 32; ++j) {
+            const float b = p.bias && j < nv ? p.bias[c0 + j] : 0.f;
+            v[j] = SCALED ? fmaf(__uint_as_float(r[j]), alpha, b) : __uint_as_float(r[j]) + b;
         }
     }
     if (p.act == ANCHA_ACT_GELU) {
@@ -193,7 +197,8 @@ __device__ __forceinline__ void finish32(const Params& p, int64_t row, bool live
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
                     const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at + j);
-                    v[j] += q.x; v[j + 1] += q.y; v[j + 2] += q.z; v[j + 3] += q.w;
+                    f2_split(fadd2(f2(v[j], v[j + 1]), f2(q.x, q.y)), v[j], v[j + 1]);
+                    f2_split(fadd2(f2(v[j + 2], v[j + 3]), f2(q.z, q.w)), v[j + 2], v[j + 3]);
                 }
             } else {
 #pragma unroll
@@ -216,9 +221,11 @@ __device__ __forceinline__ void finish32(const Params& p, int64_t row, bool live
                 if (j < nv) v[j] += residual_at(p, at + j);
         }
     }
+    if (nv < 32) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (j >= nv) v[j] = 0.f;
+        for (int j = 0; j < 32; ++j)
+            if (j >= nv) v[j] = 0.f;
+    }
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
@@ -301,30 +308,49 @@ __device__ __forceinline__ void store_plain(const Params& p, float* buf, int64_t
         store_elt(p.out, (row0 + r) * p.ldo + c0 + lane, buf[r * 32 + (lane ^ r)], p.out_type);
 }
 
-// A lane's 32 columns quantised: one block of 32, or two of 16, in its registers.
+// A lane's 32 columns quantised: one block of 32, or two of 16, in its registers. All lanes of the warp call it,
+// lane l for row row0 + l; rows from m on are not written.
 template <int FMT>
-__device__ __forceinline__ void store_mx(const MxArray& o, int okt, int64_t row, int c0, const float (&v)[32]) {
-    constexpr int B = mx_block(FMT);
+__device__ __forceinline__ void store_mx(const MxArray& o, int okt, int64_t row0, int m, int c0, int lane, const float (&v)[32]) {
+    constexpr int B = mx_block(FMT), W = FMT == MXF8 ? 8 : 4;
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
-    uint32_t codes = 0, w[8];
+    uint32_t codes = 0, w[W];
 #pragma unroll
     for (int h = 0; h < 32 / B; ++h) {
-        uint32_t a = 0;
+        float x[B], a = 0.f;
 #pragma unroll
-        for (int j = 0; j < B; ++j) a = max(a, abs_bits(v[h * B + j]));
-        const MxBlock b = mx_block_scale<FMT>(a, g);
+        for (int j = 0; j < B; ++j) x[j] = v[h * B + j];
+#pragma unroll
+        for (int j = 0; j < B; j += 2) a = absmax(a, x[j], x[j + 1]);
+        const MxBlock b = mx_block_scale<FMT>(__float_as_uint(a), g);
         codes |= b.code << (8 * h);
+        uint32_t e[W * B / 32];
+        mx_encode<FMT, B>(x, b, e);
 #pragma unroll
-        for (int j = 0; j < B; j += 2) {
-            const uint32_t q = mx_pair<FMT>(mx_scaled<FMT>(v[h * B + j], b), mx_scaled<FMT>(v[h * B + j + 1], b));
-            const int at = h * B + j;
-            if (FMT == MXF8) w[at / 4] = at % 4 ? w[at / 4] | q << 16 : q;
-            else w[at / 8] = at % 8 ? w[at / 8] | q << (at % 8 * 4) : q;
-        }
+        for (int j = 0; j < W * B / 32; ++j) w[h * (W * B / 32) + j] = e[j];
     }
-    uint8_t* d = o.data + row * o.ld + mx_bytes(FMT, c0);
-    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (FMT == MXF8 && c0 + 16 < o.cols) *reinterpret_cast<uint4*>(d + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    const int64_t row = row0 + lane;
+    if (FMT == MXF8) {
+        // Two lanes write a row's 32 bytes together, so that a store covers whole sectors: the even lane's row first,
+        // then the odd one's.
+        const bool odd = lane & 1;
+        uint4 own = make_uint4(w[0], w[1], w[2], w[3]), peer;
+        const uint4 hi = make_uint4(w[4 % W], w[5 % W], w[6 % W], w[7 % W]);
+        peer.x = __shfl_xor_sync(0xffffffffu, odd ? own.x : hi.x, 1);
+        peer.y = __shfl_xor_sync(0xffffffffu, odd ? own.y : hi.y, 1);
+        peer.z = __shfl_xor_sync(0xffffffffu, odd ? own.z : hi.z, 1);
+        peer.w = __shfl_xor_sync(0xffffffffu, odd ? own.w : hi.w, 1);
+        const int64_t even_row = row - odd;
+        uint8_t* d = o.data + even_row * o.ld + c0 + 16 * odd;
+        if (c0 + 16 * odd < o.cols) {
+            if (even_row < m) *reinterpret_cast<uint4*>(d) = odd ? peer : own;
+            if (even_row + 1 < m) *reinterpret_cast<uint4*>(d + o.ld) = odd ? hi : peer;
+        }
+    } else if (row < m) {
+        *reinterpret_cast<uint4*>(o.data + row * o.ld + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (row >= m) codes = 0;  // the scales behind the last row
+    if (row >= ((int64_t)m + 127) / 128 * 128) return;
     uint8_t* s = o.scales + mx_scale_word(row, c0 / B / 4, okt) + c0 / B % 4;
     if (B == 32) *s = (uint8_t)codes;
     else *reinterpret_cast<uint16_t*>(s) = (uint16_t)codes;
@@ -468,7 +494,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
         float alpha = 1.f;
         if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
         uint32_t local = 0;
-        bool stored = false;
+        uint32_t chunks = 0;
         for (int t = tile0; t < p.tiles; t += tstep, ++local) {
             const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
             const int b = local & 1;
@@ -499,30 +525,31 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     continue;
                 }
                 float v[32];
-                finish32(p, row, live, c0, nv, alpha, r, v);
+                finish32<FMT == NVF4>(p, row, live, c0, nv, alpha, r, v);
                 if (p.out_mode == OUT_TMA) {
-                    if (stored) {  // the store that last read this buffer is done with it
-                        if (lane == 0) bulk_wait_read<0>();
-                        __syncwarp();
+                    // 16-bit outputs alternate two halves of the buffer. The store that last read this one is done.
+                    uint8_t* buf = stage + (p.out_type != ELT_F32 && chunks % 2 ? STAGING / 2 : 0);
+                    if (lane == 0) {
+                        if (p.out_type != ELT_F32) bulk_wait_read<1>();
+                        else bulk_wait_read<0>();
                     }
-                    stage_row(stage, lane, p.out_type, v);
+                    __syncwarp();
+                    stage_row(buf, lane, p.out_type, v);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_3d(&tout, stage, c0, (int)row0, 0);
+                        tma_store_3d(&tout, buf, c0, (int)row0, 0);
                         bulk_commit();
                     }
-                    stored = true;
+                    ++chunks;
                 } else if (p.out_mode == OUT_PLAIN) {
                     store_plain(p, reinterpret_cast<float*>(stage), row0, c0, nv, lane, v);
-                } else if (!live) {
-                    zero_scales(p, row, c0);
                 } else if (p.om.format == MXF8) {
-                    store_mx<MXF8>(p.om, p.okt, row, c0, v);
+                    store_mx<MXF8>(p.om, p.okt, row0, p.m, c0, lane, v);
                 } else if (p.om.format == MXF4) {
-                    store_mx<MXF4>(p.om, p.okt, row, c0, v);
+                    store_mx<MXF4>(p.om, p.okt, row0, p.m, c0, lane, v);
                 } else {
-                    store_mx<NVF4>(p.om, p.okt, row, c0, v);
+                    store_mx<NVF4>(p.om, p.okt, row0, p.m, c0, lane, v);
                 }
             }
         }
@@ -565,17 +592,18 @@ template <int FMT>
 __device__ __forceinline__ void store_mx_lanes(const MxArray& o, int okt, int64_t row, int c0, int lane, const float (&v)[4]) {
     constexpr int B = mx_block(FMT), LB = B / 4;  // lanes of a block
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
-    uint32_t a = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+    uint32_t a = __float_as_uint(absmax(absmax(0.f, v[0], v[1]), v[2], v[3]));
 #pragma unroll
     for (int d = 1; d < LB; d *= 2) a = max(a, __shfl_xor_sync(0xffffffffu, a, d));
     const MxBlock b = mx_block_scale<FMT>(a, g);
-    const uint32_t lo = mx_pair<FMT>(mx_scaled<FMT>(v[0], b), mx_scaled<FMT>(v[1], b));
-    const uint32_t hi = mx_pair<FMT>(mx_scaled<FMT>(v[2], b), mx_scaled<FMT>(v[3], b));
+    float x[8] = {v[0], v[1], v[2], v[3]};
+    uint32_t w[FMT == MXF8 ? 2 : 1];
+    mx_encode<FMT, 8>(x, b, w);
     const int c = c0 + 4 * lane;
     if (mx_bytes(FMT, c) < mx_row_bytes(FMT, o.cols)) {
         uint8_t* d = o.data + row * o.ld + mx_bytes(FMT, c);
-        if (FMT == MXF8) *reinterpret_cast<uint32_t*>(d) = lo | hi << 16;
-        else *reinterpret_cast<uint16_t*>(d) = (uint16_t)(lo | hi << 8);
+        if (FMT == MXF8) *reinterpret_cast<uint32_t*>(d) = w[0];
+        else *reinterpret_cast<uint16_t*>(d) = (uint16_t)w[0];
     }
     if (lane % LB == 0 && c / B < 4 * okt) o.scales[mx_scale_word(row, c / B / 4, okt) + c / B % 4] = (uint8_t)b.code;
 }
@@ -829,7 +857,7 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
 template <int FMT>
 int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
     const int64_t row_tiles = p.m <= 64 ? 1 : ceil_div(p.m, 128), tiles = row_tiles * ceil_div(p.n, 128);
-    if (p.m <= 64 || tiles <= 74) {
+    if (p.m <= 64 || tiles <= 300) {
         const int slabs = (int)ceil_div(p.kbytes, SLAB);
         int splits = 1;
         while (splits < 8 && 2 * splits <= slabs && tiles * 2 * splits <= 296) splits *= 2;
@@ -853,6 +881,7 @@ int mx_linear(const MxLinear& q, cudaStream_t s) {
     p.bias = q.bias;
     p.residual = q.residual; p.ldr = q.ldr; p.res_type = q.res_type;
     p.res_vec = q.residual && aligned16(q.residual) && q.ldr * (int64_t)elt_size(q.res_type) % 16 == 0;
+    p.bias_vec = aligned16(q.bias);
     p.act = q.act;
     p.out = q.out; p.ldo = q.ldo; p.out_type = q.out_type;
     if (q.out_mx) {

@@ -82,9 +82,7 @@ template <int FMT>
 __device__ __forceinline__ void quantize8(const float (&v)[8], int c, int64_t row, int cols, int64_t kt, uint8_t* data,
                                           int64_t ld, uint8_t* scales, float global, bool store) {
     constexpr int LB = block_lanes<FMT>();
-    uint32_t a = abs_bits(v[0]);
-#pragma unroll
-    for (int j = 1; j < 8; ++j) a = max(a, abs_bits(v[j]));
+    uint32_t a = __float_as_uint(absmax(absmax(absmax(absmax(0.f, v[0], v[1]), v[2], v[3]), v[4], v[5]), v[6], v[7]));
 #pragma unroll
     for (int o = 1; o < LB; o *= 2) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
     const MxBlock b = mx_block_scale<FMT>(a, global);
@@ -93,16 +91,15 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], int c, int64_t ro
     word |= __shfl_xor_sync(0xffffffffu, word, LB);
     word |= __shfl_xor_sync(0xffffffffu, word, 2 * LB);
     if (!store) return;
-    uint32_t p[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = mx_pair<FMT>(mx_scaled<FMT>(v[2 * j], b), mx_scaled<FMT>(v[2 * j + 1], b));
+    uint32_t w[FMT == MXF8 ? 2 : 1];
+    mx_encode<FMT, 8>(v, b, w);
     const int64_t at = mx_bytes(FMT, c);
     if (at < mx_row_bytes(FMT, cols)) {
         uint8_t* d = data + row * ld + at;
-        if (FMT == MXF8)
-            *reinterpret_cast<uint2*>(d) = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+        if constexpr (FMT == MXF8)
+            *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
         else
-            *reinterpret_cast<uint32_t*>(d) = p[0] | p[1] << 8 | p[2] << 16 | p[3] << 24;
+            *reinterpret_cast<uint32_t*>(d) = w[0];
     }
     if (lane % word_lanes<FMT>() == 0)
         *reinterpret_cast<uint32_t*>(scales + mx_scale_word(row, c / (4 * mx_block(FMT)), kt)) = word;
