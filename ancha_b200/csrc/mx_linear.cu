@@ -365,6 +365,11 @@ __device__ __forceinline__ void zero_scales(const Params& p, int64_t row, int c0
     else *reinterpret_cast<uint16_t*>(s) = 0;
 }
 
+// A converged warp's wait; false where one lane's ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err));
+}
+
 template <int FMT, int BN, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
@@ -460,31 +465,36 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t idesc = idesc_of<FMT>(BMT, BN);
             uint32_t it = 0, local = 0;
             for (int t = tile0; t < p.tiles && !*abort; t += tstep, ++local) {
                 const int b = local & 1;
                 if (S::SHARED_COLS) {
-                    if (local && !mbar_wait(&tempty[0], (local - 1) & 1, abort, p.err)) break;
-                } else if (!mbar_wait(&tempty[b], ((local >> 1) & 1) ^ 1, abort, p.err)) {
+                    if (local && !warp_wait(&tempty[0], (local - 1) & 1, abort, p.err)) break;
+                } else if (!warp_wait(&tempty[b], ((local >> 1) & 1) ^ 1, abort, p.err)) {
                     break;
                 }
                 tc_fence_after();
                 const uint32_t acc = tmem + b * S::ACC1;
                 for (int kb = 0; kb < slabs; ++kb, ++it) {
                     const int s = it % STAGES;
-                    if (!mbar_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
+                    if (!warp_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
                     tc_fence_after();
                     const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
-                    slab_products<FMT, PAIR, BN>(acc, tmem + SFA_COL, tmem + SFB_COL, smem_u32(a_tiles + s * OPERAND_BYTES),
-                                                 smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
-                                                 smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0);
-                    if (PAIR) umma_commit_pair(&empty[s], 0x3);
-                    else umma_commit(&empty[s]);
+                    if (elect_one()) {
+                        slab_products<FMT, PAIR, BN>(acc, tmem + SFA_COL, tmem + SFB_COL, smem_u32(a_tiles + s * OPERAND_BYTES),
+                                                     smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
+                                                     smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0);
+                        if (PAIR) umma_commit_pair(&empty[s], 0x3);
+                        else umma_commit(&empty[s]);
+                        if (kb == slabs - 1) {
+                            if (PAIR) umma_commit_pair(&tfull[b], 0x3);
+                            else umma_commit(&tfull[b]);
+                        }
+                    }
+                    __syncwarp();
                 }
-                if (PAIR) umma_commit_pair(&tfull[b], 0x3);
-                else umma_commit(&tfull[b]);
             }
         }
     } else {
@@ -685,22 +695,22 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_of<FMT>(BM, TN);
-            uint32_t it = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % STAGES;
-                if (!mbar_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
-                tc_fence_after();
-                const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
+        constexpr uint32_t idesc = idesc_of<FMT>(BM, TN);
+        uint32_t it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % STAGES;
+            if (!warp_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
+            tc_fence_after();
+            const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
+            if (elect_one()) {
                 slab_products<FMT, false, TN>(tmem, tmem + TN, tmem + TN + 4 * S::SF, smem_u32(w_tiles + s * OPERAND_BYTES),
                                               smem_u32(x_tiles + s * TN * SLAB), smem_u32(sw_tiles + s * S::SF * SF_TILE),
                                               smem_u32(sx_tiles + s * S::SF * SF_TILE), idesc, steps, kb == kb0);
                 umma_commit(&empty[s]);
+                if (kb == kb1 - 1) umma_commit(done);
             }
-            umma_commit(done);
+            __syncwarp();
         }
-        __syncwarp();
     }
     const int live = min(TN, p.m - m0);  // rows of x in the tile
     if (warp >= 2) {

@@ -172,6 +172,15 @@ __device__ __forceinline__ void prefetch_tma(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// True in one lane of a converged warp, the same one every time. The compiler knows that a branch on it
+// leaves one thread, so the tcgen05 instructions behind it take their operands (uniform registers) directly; behind
+// `lane == 0` it emits a loop over the lanes for each of them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+
 // TMEM allocation (whole warp).
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
