@@ -22,9 +22,8 @@ namespace {
 constexpr int BM = 128, SLAB = 128;          // rows of a CTA's tile, bytes of a K slab
 constexpr int OPERAND_BYTES = BM * SLAB;     // 128 rows of a slab
 constexpr int SF_TILE = 512;                 // a scale tile
-constexpr int EPI = 16;                      // epilogue warps
-constexpr int THREADS = 64 + 32 * EPI;
 constexpr int STAGING = 4096;                // per epilogue warp: 32 rows x 128 bytes
+constexpr int BIAS_BYTES = 256;              // and the bias of its 64 columns
 // TMEM: two accumulators, then the scales of the slab in work.
 constexpr uint32_t SFA_COL = 448, SFB_COL = 464, TMEM_COLS = 512;
 
@@ -35,11 +34,13 @@ struct Shape {
     static constexpr int SF = sf_tiles(FMT);
     static constexpr int B_ROWS = PAIR ? BN / 2 : BN;   // w's rows in this CTA
     static constexpr int B_BYTES = B_ROWS * SLAB;
-    static constexpr int SFA_BYTES = SF * SF_TILE, SFB_BYTES = SF * SF_TILE * (BN / 128);
+    static constexpr int RANGES = (BN + 127) / 128;     // 128-row ranges of w's scales
+    static constexpr int SFA_BYTES = SF * SF_TILE, SFB_BYTES = SF * SF_TILE * RANGES;
     static constexpr int STAGE = OPERAND_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int STAGES = (227 * 1024 - 1024 - 256 - EPI * STAGING) / STAGE < 6
-                                      ? (227 * 1024 - 1024 - 256 - EPI * STAGING) / STAGE : 6;
-    static constexpr int BYTES = 1024 + STAGES * STAGE + EPI * STAGING + 256;
+    static constexpr int EPI = BN / 16;                 // epilogue warps: 32 rows by 64 columns of the tile each
+    static constexpr int THREADS = 64 + 32 * EPI;
+    static constexpr int FIT = (227 * 1024 - 1024 - 256 - EPI * (STAGING + BIAS_BYTES)) / STAGE, STAGES = FIT < 6 ? FIT : 6;
+    static constexpr int BYTES = 1024 + STAGES * STAGE + EPI * (STAGING + BIAS_BYTES) + 256;
     // Second accumulator. Two of 256 columns and the scales do not fit 512: they share 64 columns, which
     // the epilogue of a tile drains first, so the next tile's products start when those are free.
     static constexpr uint32_t ACC1 = BN == 256 ? 192 : BN;
@@ -54,7 +55,7 @@ struct Params {
     const float* bias;
     const void* residual;
     int64_t ldr;
-    int res_type, res_vec, bias_vec, act;
+    int res_type, res_vec, act;
     void* out;
     int64_t ldo;
     int out_type, out_mode;    // OUT_*
@@ -111,12 +112,13 @@ __host__ __device__ constexpr uint32_t idesc_of(int m, int n) {
 
 // The products of one slab: `steps` (1 to 4) K steps of 32 bytes. Step i takes scale tile i / (4 / SF) and in
 // it the byte (1X), byte pair (2X) or all four bytes (4X) of its blocks. sfa, sfb: TMEM columns of the scales
-// (4 SF, and 4 SF for each 128 columns of the tile or part of them).
+// (4 SF, and 4 SF for each 128 columns of the tile or part of them); sfb_skip: columns of the latter before the
+// tile's first.
 template <int FMT, bool PAIR, int BN>
 __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32_t sfb, uint32_t a, uint32_t b, uint32_t sa,
-                                              uint32_t sb, uint32_t idesc, int steps, bool first) {
+                                              uint32_t sb, uint32_t idesc, int steps, bool first, uint32_t sfb_skip = 0) {
     constexpr int SF = sf_tiles(FMT), PER = 4 / SF;  // K steps per scale tile
-    constexpr int RANGES = BN > 128 ? BN / 128 : 1;  // 128-row ranges of w's scales
+    constexpr int RANGES = (BN + 127) / 128;  // 128-row ranges of w's scales
 #pragma unroll
     for (int t = 0; t < SF; ++t) {
         if (t * PER >= steps) break;
@@ -131,7 +133,7 @@ __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32
         const int t = i / PER;
         const uint32_t id = FMT == MXF8 ? i : FMT == MXF4 ? i % 2 * 2 : 0;
         mma<FMT, PAIR>(acc, umma_desc_sw128(a + i * 32), umma_desc_sw128(b + i * 32), idesc | id << 4 | id << 29,
-                       sfa + 4 * t, sfb + 4 * t * RANGES, !(first && i == 0));
+                       sfa + 4 * t, sfb + 4 * t * RANGES + sfb_skip, !(first && i == 0));
     }
 }
 
@@ -161,27 +163,20 @@ __device__ __forceinline__ float residual_at(const Params& p, int64_t i) {
                                     : __half2float(static_cast<const __half*>(p.residual)[i]);
 }
 
-// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them). The arithmetic
+// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them); `bias`: theirs, in shared
+// memory. The arithmetic
 // runs on packed pairs, one instruction for two values: the epilogue is bound by instruction issue.
 template <bool SCALED>
-__device__ __forceinline__ void finish32(const Params& p, int64_t row, bool live, int c0, int nv, float alpha,
-                                         const uint32_t (&r)[32], float (&v)[32]) {
+__device__ __forceinline__ void finish32(const Params& p, const float* bias, int64_t row, bool live, int c0, int nv,
+                                         float alpha, const uint32_t (&r)[32], float (&v)[32]) {
     const uint64_t al = f2(alpha, alpha);
-    if (p.bias && p.bias_vec && nv == 32) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(p.bias + c0 + j);
-            const uint64_t a = f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-            const uint64_t b = f2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-            f2_split(SCALED ? ffma2(a, al, f2(q.x, q.y)) : fadd2(a, f2(q.x, q.y)), v[j], v[j + 1]);
-            f2_split(SCALED ? ffma2(b, al, f2(q.z, q.w)) : fadd2(b, f2(q.z, q.w)), v[j + 2], v[j + 3]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float b = p.bias && j < nv ? p.bias[c0 + j] : 0.f;
-            v[j] = SCALED ? fmaf(__uint_as_float(r[j]), alpha, b) : __uint_as_float(r[j]) + b;
-        }
+    for (int j = 0; j < 32; j += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(bias + j);
+        const uint64_t a = f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+        const uint64_t b = f2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+        f2_split(SCALED ? ffma2(a, al, f2(q.x, q.y)) : fadd2(a, f2(q.x, q.y)), v[j], v[j + 1]);
+        f2_split(SCALED ? ffma2(b, al, f2(q.z, q.w)) : fadd2(b, f2(q.z, q.w)), v[j + 2], v[j + 3]);
     }
     if (p.act == ANCHA_ACT_GELU) {
 #pragma unroll
@@ -278,18 +273,18 @@ __device__ __forceinline__ void store4(void* base, int type, bool vec, int64_t a
         if (j < nv) store_elt(base, at + j, v[j], type);
 }
 
-// A lane's row of 32 values in the swizzled staging layout of the TMA store (128-byte rows of f32 with the
-// 128-byte swizzle, 64-byte rows of 16 bits with the 64-byte swizzle).
-__device__ __forceinline__ void stage_row(uint8_t* buf, int lane, int type, const float (&v)[32]) {
+// A lane's row of 32 values in a staging buffer of 128-byte rows with the 128-byte swizzle: 32 columns of f32, or
+// half `h` of 64 columns of 16 bits.
+__device__ __forceinline__ void stage_row(uint8_t* buf, int lane, int type, int h, const float (&v)[32]) {
+    buf += lane * 128;
     if (type == ELT_F32) {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) =
-                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            *reinterpret_cast<float4*>(buf + ((q ^ (lane & 7)) * 16)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
+            *reinterpret_cast<uint4*>(buf + (((q + 4 * h) ^ (lane & 7)) * 16)) =
                 make_uint4(pack16(v[8 * q], v[8 * q + 1], type), pack16(v[8 * q + 2], v[8 * q + 3], type),
                            pack16(v[8 * q + 4], v[8 * q + 5], type), pack16(v[8 * q + 6], v[8 * q + 7], type));
     }
@@ -310,8 +305,9 @@ __device__ __forceinline__ void store_plain(const Params& p, float* buf, int64_t
 
 // A lane's 32 columns quantised: one block of 32, or two of 16, in its registers. All lanes of the warp call it,
 // lane l for row row0 + l; rows from m on are not written.
+// Returns the scale code, or the two.
 template <int FMT>
-__device__ __forceinline__ void store_mx(const MxArray& o, int okt, int64_t row0, int m, int c0, int lane, const float (&v)[32]) {
+__device__ __forceinline__ uint32_t store_mx(const MxArray& o, int64_t row0, int m, int c0, int lane, const float (&v)[32]) {
     constexpr int B = mx_block(FMT), W = FMT == MXF8 ? 8 : 4;
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
     uint32_t codes = 0, w[W];
@@ -349,20 +345,7 @@ __device__ __forceinline__ void store_mx(const MxArray& o, int okt, int64_t row0
     } else if (row < m) {
         *reinterpret_cast<uint4*>(o.data + row * o.ld + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (row >= m) codes = 0;  // the scales behind the last row
-    if (row >= ((int64_t)m + 127) / 128 * 128) return;
-    uint8_t* s = o.scales + mx_scale_word(row, c0 / B / 4, okt) + c0 / B % 4;
-    if (B == 32) *s = (uint8_t)codes;
-    else *reinterpret_cast<uint16_t*>(s) = (uint16_t)codes;
-}
-
-// Scales of a chunk that lies behind the last row or column, inside the last scale tiles: 0.
-__device__ __forceinline__ void zero_scales(const Params& p, int64_t row, int c0) {
-    const int b = mx_block(p.om.format);
-    if (row >= ((int64_t)p.m + 127) / 128 * 128 || c0 / (4 * b) >= p.okt) return;
-    uint8_t* s = p.om.scales + mx_scale_word(row, c0 / b / 4, p.okt) + c0 / b % 4;
-    if (b == 32) *s = 0;
-    else *reinterpret_cast<uint16_t*>(s) = 0;
+    return codes;
 }
 
 // A converged warp's wait; false where one lane's ran out.
@@ -371,18 +354,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 template <int FMT, int BN, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Shape<FMT, BN, PAIR>::THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
               const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
               const __grid_constant__ CUtensorMap tout, const __grid_constant__ Params p) {
     using S = Shape<FMT, BN, PAIR>;
-    constexpr int BMT = PAIR ? 2 * BM : BM, STAGES = S::STAGES;
+    constexpr int BMT = PAIR ? 2 * BM : BM, STAGES = S::STAGES, EPI = S::EPI;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* a_tiles = smem;
     uint8_t* b_tiles = a_tiles + STAGES * OPERAND_BYTES;
     uint8_t* staging = b_tiles + STAGES * S::B_BYTES;  // 1024-byte aligned, as the operands
-    uint8_t* sa_tiles = staging + EPI * STAGING;
+    uint8_t* sa_tiles = staging + EPI * (STAGING + BIAS_BYTES);
     uint8_t* sb_tiles = sa_tiles + STAGES * S::SFA_BYTES;
     uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + STAGES * S::SFB_BYTES);
     uint64_t* empty = full + STAGES;
@@ -429,13 +412,13 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     const int slabs = (p.kbytes + SLAB - 1) / SLAB;
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int t = tile0; t < p.tiles && !*abort; t += tstep) {
-                const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
-                for (int kb = 0; kb < slabs; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+        uint32_t it = 0;
+        for (int t = tile0; t < p.tiles && !*abort; t += tstep) {
+            const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
+            for (int kb = 0; kb < slabs; ++kb, ++it) {
+                const int s = it % STAGES;
+                if (!warp_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+                if (elect_one()) {
                     uint8_t* a = a_tiles + s * OPERAND_BYTES;
                     uint8_t* b = b_tiles + s * S::B_BYTES;
                     uint8_t* sa = sa_tiles + s * S::SFA_BYTES;
@@ -456,14 +439,16 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                         tma_load_3d(sb, &tsb, &full[s], 0, kb * S::SF * 2, n0 / 128);
                     }
                 }
-            }
-            if (*abort && rank == 0) {  // let copies in flight land before the CTA exits (bounded)
-                const long long c0 = clock64();
-                for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
-                    while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
-                    }
+                __syncwarp();
             }
         }
+        if (*abort && rank == 0 && lane == 0) {  // let copies in flight land before the CTA exits (bounded)
+            const long long c0 = clock64();
+            for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
+                while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
+                }
+        }
+        __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
             constexpr uint32_t idesc = idesc_of<FMT>(BMT, BN);
@@ -485,7 +470,8 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     if (elect_one()) {
                         slab_products<FMT, PAIR, BN>(acc, tmem + SFA_COL, tmem + SFB_COL, smem_u32(a_tiles + s * OPERAND_BYTES),
                                                      smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
-                                                     smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0);
+                                                     smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0,
+                                                     BN == 192 ? (uint32_t)(t % p.n_tiles & 1) * 2 : 0);
                         if (PAIR) umma_commit_pair(&empty[s], 0x3);
                         else umma_commit(&empty[s]);
                         if (kb == slabs - 1) {
@@ -498,72 +484,94 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             }
         }
     } else {
-        constexpr int PER_QUARTER = EPI / 4, CHUNKS = BN / 32;
-        const int quarter = warp % 4, first = (warp - 2) / 4;
+        const int quarter = warp % 4, col0 = (warp - 2) / 4 * 64;
         uint8_t* stage = staging + (warp - 2) * STAGING;
+        float* bias = reinterpret_cast<float*>(staging + EPI * STAGING) + (warp - 2) * 64;
         float alpha = 1.f;
         if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
+        const bool wide = p.out_type == ELT_F32;
         uint32_t local = 0;
-        uint32_t chunks = 0;
         for (int t = tile0; t < p.tiles; t += tstep, ++local) {
-            const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
+            const int m0 = t / p.n_tiles * BMT, c_first = t % p.n_tiles * BN + col0;
             const int b = local & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(&tfull[b], (local >> 1) & 1, abort, p.err))) break;
+            // The tile's bias, on its way while the products run: read in the epilogue it would cost each chunk the
+            // latency of L2.
+            float b0 = 0.f, b1 = 0.f;
+            if (p.bias) {
+                if (c_first + lane < p.n) b0 = p.bias[c_first + lane];
+                if (c_first + 32 + lane < p.n) b1 = p.bias[c_first + 32 + lane];
+            }
+            __syncwarp();
+            bias[lane] = b0;
+            bias[32 + lane] = b1;
+            if (!warp_wait(&tfull[b], (local >> 1) & 1, abort, p.err)) break;
             tc_fence_after();
             const int64_t row0 = m0 + (int)rank * BM + quarter * 32, row = row0 + lane;
-            const bool live = row < p.m;
-            const uint32_t base = tmem + b * S::ACC1 + ((uint32_t)(quarter * 32) << 16);
+            const bool some = row0 < p.m && c_first < p.n;
+            const uint32_t base = tmem + b * S::ACC1 + col0 + ((uint32_t)(quarter * 32) << 16);
+            uint32_t codes = 0;
 #pragma unroll 1
-            for (int o = first; o < CHUNKS; o += PER_QUARTER) {
-                // The shared columns, the last two chunks of one accumulator and the first two of the other, first.
-                const int col = 32 * (S::SHARED_COLS && b == 0 ? (o + CHUNKS - 2) % CHUNKS : o);
+            for (int h = 0; h < 2; ++h) {
                 uint32_t r[32];
-                tmem_ld32(base + col, r);
+                tmem_ld32(base + 32 * h, r);
                 tmem_wait_ld();
-                if (S::SHARED_COLS ? o == first : o + PER_QUARTER >= CHUNKS) {
+                if (h == 1) {  // this warp is done with the accumulator (and with every earlier one)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
-                        if (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0));
+                        if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0));
                         else mbar_arrive(bar);
                     }
                 }
-                const int c0 = n0 + col, nv = min(32, p.n - c0);
-                if (nv <= 0 || row0 >= p.m) {
-                    if (p.out_mode == OUT_MX) zero_scales(p, row, c0);
-                    continue;
-                }
+                const int c0 = c_first + 32 * h, nv = min(32, p.n - c0);
+                if (nv <= 0 || !some) continue;
                 float v[32];
-                finish32<FMT == NVF4>(p, row, live, c0, nv, alpha, r, v);
+                finish32<FMT == NVF4>(p, bias + 32 * h, row, row < p.m, c0, nv, alpha, r, v);
                 if (p.out_mode == OUT_TMA) {
-                    // 16-bit outputs alternate two halves of the buffer. The store that last read this one is done.
-                    uint8_t* buf = stage + (p.out_type != ELT_F32 && chunks % 2 ? STAGING / 2 : 0);
-                    if (lane == 0) {
-                        if (p.out_type != ELT_F32) bulk_wait_read<1>();
-                        else bulk_wait_read<0>();
+                    if (wide || h == 0) {  // the store that last read the buffer is done with it
+                        if (elect_one()) bulk_wait_read<0>();
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    stage_row(buf, lane, p.out_type, v);
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_3d(&tout, buf, c0, (int)row0, 0);
-                        bulk_commit();
+                    stage_row(stage, lane, p.out_type, h, v);
+                    if (wide) {
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (elect_one()) {
+                            tma_store_3d(&tout, stage, c0, (int)row0, 0);
+                            bulk_commit();
+                        }
                     }
-                    ++chunks;
                 } else if (p.out_mode == OUT_PLAIN) {
                     store_plain(p, reinterpret_cast<float*>(stage), row0, c0, nv, lane, v);
                 } else if (p.om.format == MXF8) {
-                    store_mx<MXF8>(p.om, p.okt, row0, p.m, c0, lane, v);
+                    codes |= store_mx<MXF8>(p.om, row0, p.m, c0, lane, v) << (8 * h);
                 } else if (p.om.format == MXF4) {
-                    store_mx<MXF4>(p.om, p.okt, row0, p.m, c0, lane, v);
+                    codes |= store_mx<MXF4>(p.om, row0, p.m, c0, lane, v) << (8 * h);
                 } else {
-                    store_mx<NVF4>(p.om, p.okt, row0, p.m, c0, lane, v);
+                    codes |= store_mx<NVF4>(p.om, row0, p.m, c0, lane, v) << (16 * h);
+                }
+            }
+            if (p.out_mode == OUT_TMA && !wide && some) {
+                fence_proxy_async();
+                __syncwarp();
+                if (elect_one()) {
+                    tma_store_3d(&tout, stage, c_first, (int)row0, 0);
+                    bulk_commit();
+                }
+            }
+            if (p.out_mode == OUT_MX) {
+                // The scales of 64 columns; 0 behind the last row and column, as far as the scale tiles reach.
+                const int block = mx_block(p.om.format), blk = c_first / block;
+                if (row < ((int64_t)p.m + 127) / 128 * 128 && blk / 4 < p.okt) {
+                    uint8_t* sc = p.om.scales + mx_scale_word(row, blk / 4, p.okt) + blk % 4;
+                    if (row >= p.m) codes = 0;
+                    if (block == 32) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)codes;
+                    else *reinterpret_cast<uint32_t*>(sc) = codes;
                 }
             }
         }
-        if (lane == 0) bulk_wait<0>();
+        if (elect_one()) bulk_wait<0>();
         __syncwarp();
     }
     tc_fence_before();
@@ -675,23 +683,24 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
     const int kb0 = (int)((int64_t)slabs * rank / splits), kb1 = (int)((int64_t)slabs * (rank + 1) / splits);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % STAGES;
-                if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+        uint32_t it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % STAGES;
+            if (!warp_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+            if (elect_one()) {
                 mbar_arrive_expect_tx(&full[s], S::STAGE);
                 tma_load_3d(w_tiles + s * OPERAND_BYTES, &tw, &full[s], kb * SLAB, n0, 0);
                 tma_load_3d(sw_tiles + s * S::SF * SF_TILE, &tsw, &full[s], 0, kb * S::SF * 2, n0 / 128);
                 tma_load_3d(x_tiles + s * TN * SLAB, &tx, &full[s], kb * SLAB, m0, 0);
                 tma_load_3d(sx_tiles + s * S::SF * SF_TILE, &tsx, &full[s], 0, kb * S::SF * 2, m0 / 128);
             }
-            if (*abort) {  // let copies in flight land before the CTA exits (bounded)
-                const long long c0 = clock64();
-                for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
-                    while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
-                    }
-            }
+            __syncwarp();
+        }
+        if (*abort && lane == 0) {  // let copies in flight land before the CTA exits (bounded)
+            const long long c0 = clock64();
+            for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
+                while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
+                }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -827,7 +836,7 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.blockDim = dim3(S::THREADS, 1, 1);
     cfg.dynamicSmemBytes = S::BYTES;
     cfg.attrs = attr;
     cfg.numAttrs = PAIR ? 1 : 0;
@@ -848,10 +857,10 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     ANCHA_TRY(make_tma_bytes(&ta, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, BM, true));
     ANCHA_TRY(make_tma_bytes(&tb, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, S::B_ROWS, true));
     ANCHA_TRY(make_tma_scales(&tsa, q.x.scales, akt, ceil_div(p.m, 128), S::SF, 1));
-    ANCHA_TRY(make_tma_scales(&tsb, q.w.scales, akt, ceil_div(p.n, 128), S::SF, BN / 128));
+    ANCHA_TRY(make_tma_scales(&tsb, q.w.scales, akt, ceil_div(p.n, 128), S::SF, S::RANGES));
     to = ta;
     if (p.out_mode == OUT_TMA)
-        ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, 32, 32));
+        ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, p.out_type == ELT_F32 ? 32 : 64, 32));
     p.m_tiles = (int)ceil_div(p.m, PAIR ? 2 * BM : BM);
     p.n_tiles = (int)ceil_div(p.n, BN);
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
@@ -875,7 +884,11 @@ int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
         if (p.m <= 64) return launch_split<FMT, 64>(q, p, splits, s);
         return launch_split<FMT, 128>(q, p, splits, s);
     }
-    if (p.m > 128 && p.n > 128) return launch<FMT, 256, true>(q, p, s);
+    if (p.m > 128 && p.n > 128) {
+        // The tile width that pads n less.
+        if (ceil_div(p.n, 192) * 192 < ceil_div(p.n, 256) * 256) return launch<FMT, 192, true>(q, p, s);
+        return launch<FMT, 256, true>(q, p, s);
+    }
     return launch<FMT, 128, false>(q, p, s);
 }
 
@@ -891,7 +904,6 @@ int mx_linear(const MxLinear& q, cudaStream_t s) {
     p.bias = q.bias;
     p.residual = q.residual; p.ldr = q.ldr; p.res_type = q.res_type;
     p.res_vec = q.residual && aligned16(q.residual) && q.ldr * (int64_t)elt_size(q.res_type) % 16 == 0;
-    p.bias_vec = aligned16(q.bias);
     p.act = q.act;
     p.out = q.out; p.ldo = q.ldo; p.out_type = q.out_type;
     if (q.out_mx) {
