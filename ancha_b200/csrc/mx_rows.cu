@@ -28,58 +28,120 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
-// Sixteen elements of a row from column c (a multiple of 16), zeros from column `cols` on. `vec`: the row starts on a
-// 16-byte boundary.
-__device__ __forceinline__ void load16(const void* row, int dtype, bool vec, int c, int cols, float (&v)[PER]) {
-    if (vec && c + PER <= cols) {
-        if (dtype == ELT_F32) {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 q = p[j];
-                v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
-            }
-        } else {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
-            const uint4 q[2] = {p[0], p[1]};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                unpack16(q[j].x, dtype, v[8 * j], v[8 * j + 1]);
-                unpack16(q[j].y, dtype, v[8 * j + 2], v[8 * j + 3]);
-                unpack16(q[j].z, dtype, v[8 * j + 4], v[8 * j + 5]);
-                unpack16(q[j].w, dtype, v[8 * j + 6], v[8 * j + 7]);
-            }
-        }
-        return;
+__device__ __forceinline__ float element(const void* row, int dtype, int c) {
+    return dtype == ELT_F32    ? static_cast<const float*>(row)[c]
+           : dtype == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(row)[c])
+                               : __half2float(static_cast<const __half*>(row)[c]);
+}
+
+// How a row's address allows it to be reached: an element at a time, in 16-byte or in 32-byte pieces.
+enum : int { BY_ELEMENT = 0, BY_16 = 1, BY_32 = 2 };
+
+struct Words8 {
+    uint32_t w[8];
+};
+__device__ __forceinline__ Words8 ld32(const void* p, int access) {
+    Words8 q;
+    if (access == BY_32) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(q.w[0]), "=r"(q.w[1]), "=r"(q.w[2]), "=r"(q.w[3]), "=r"(q.w[4]), "=r"(q.w[5]), "=r"(q.w[6]),
+                       "=r"(q.w[7])
+                     : "l"(p)
+                     : "memory");
+    } else {
+        const uint4 a = static_cast<const uint4*>(p)[0], b = static_cast<const uint4*>(p)[1];
+        q = {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        v[j] = 0.f;
-        if (c + j < cols)
-            v[j] = dtype == ELT_F32    ? static_cast<const float*>(row)[c + j]
-                   : dtype == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(row)[c + j])
-                                       : __half2float(static_cast<const __half*>(row)[c + j]);
+    return q;
+}
+__device__ __forceinline__ void st32(void* p, int access, const Words8& q) {
+    if (access == BY_32) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(q.w[0]), "r"(q.w[1]), "r"(q.w[2]),
+                     "r"(q.w[3]), "r"(q.w[4]), "r"(q.w[5]), "r"(q.w[6]), "r"(q.w[7])
+                     : "memory");
+    } else {
+        static_cast<uint4*>(p)[0] = make_uint4(q.w[0], q.w[1], q.w[2], q.w[3]);
+        static_cast<uint4*>(p)[1] = make_uint4(q.w[4], q.w[5], q.w[6], q.w[7]);
     }
 }
 
-__device__ __forceinline__ void store16(void* row, int dtype, bool vec, int c, int cols, const float (&v)[PER]) {
-    if (vec && c + PER <= cols) {
-        if (dtype == ELT_F32) {
-            float4* p = reinterpret_cast<float4*>(static_cast<float*>(row) + c);
+// Slot of element e (0 .. 511) of a warp's exchange buffer: lanes reading sixteen consecutive ones and lanes reading
+// neighbours both meet 32 banks.
+constexpr int EXCHANGE = 512 + 32;
+__device__ __forceinline__ int slot(int e) { return e + (e >> 4); }
+
+// Sixteen elements of a row from column c (a multiple of 16) for every lane, zeros from column `cols` on (cols 0: a lane
+// without a row). GROUP neighbouring lanes hold neighbouring chunks of one row; where its address allows no vector loads
+// they read neighbouring elements together and exchange them through `buf` (a warp's). All lanes of the warp call it.
+template <int GROUP>
+__device__ __forceinline__ void load16(const void* row, int dtype, int access, int c, int cols, float* buf, float (&v)[PER]) {
+    if (access != BY_ELEMENT) {
+        if (c + PER <= cols) {
+            if (dtype == ELT_F32) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        } else {
-            uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + c);
+                for (int h = 0; h < 2; ++h) {
+                    const Words8 q = ld32(static_cast<const float*>(row) + c + 8 * h, access);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                p[j] = make_uint4(pack16(v[8 * j], v[8 * j + 1], dtype), pack16(v[8 * j + 2], v[8 * j + 3], dtype),
-                                  pack16(v[8 * j + 4], v[8 * j + 5], dtype), pack16(v[8 * j + 6], v[8 * j + 7], dtype));
+                    for (int j = 0; j < 8; ++j) v[8 * h + j] = __uint_as_float(q.w[j]);
+                }
+            } else {
+                const Words8 q = ld32(static_cast<const uint16_t*>(row) + c, access);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) unpack16(q.w[j], dtype, v[2 * j], v[2 * j + 1]);
+            }
+            return;
         }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = c + j < cols ? element(row, dtype, c + j) : 0.f;
         return;
     }
+    const int lane = threadIdx.x % 32, sub = lane % GROUP, base = (lane - sub) * PER;
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-        if (c + j < cols) store_elt(row, c + j, v[j], dtype);
+    for (int k = 0; k < PER; ++k) {
+        const int col = c - sub * PER + k * GROUP + sub;
+        buf[slot(base + k * GROUP + sub)] = col < cols ? element(row, dtype, col) : 0.f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = buf[slot(lane * PER + j)];
+}
+
+// The way back; columns from `cols` on are not written.
+template <int GROUP>
+__device__ __forceinline__ void store16(void* row, int dtype, int access, int c, int cols, float* buf, const float (&v)[PER]) {
+    if (access != BY_ELEMENT) {
+        if (c + PER <= cols) {
+            Words8 q;
+            if (dtype == ELT_F32) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q.w[j] = __float_as_uint(v[8 * h + j]);
+                    st32(static_cast<float*>(row) + c + 8 * h, access, q);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q.w[j] = pack16(v[2 * j], v[2 * j + 1], dtype);
+                st32(static_cast<uint16_t*>(row) + c, access, q);
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (c + j < cols) store_elt(row, c + j, v[j], dtype);
+        return;
+    }
+    const int lane = threadIdx.x % 32, sub = lane % GROUP, base = (lane - sub) * PER;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) buf[slot(lane * PER + j)] = v[j];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int col = c - sub * PER + k * GROUP + sub;
+        if (col < cols) store_elt(row, col, buf[slot(base + k * GROUP + sub)], dtype);
+    }
 }
 
 // n / d for n < 2^31 by a multiplication (d >= 1; Granlund and Montgomery's round-up method).
@@ -135,7 +197,7 @@ __device__ __forceinline__ void quantize16(const float (&v)[PER], int c, int64_t
 // One scale word (128 elements, 64 for NVF4) per eight (four) lanes; the rows up to the end of the last scale
 // tile are walked too, for their zero scales. `first`: the launch's first word.
 template <int FMT>
-__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int dtype, int vec, int64_t ldx,
+__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int dtype, int access, int64_t ldx,
                                                        const __grid_constant__ MxArray o, FastDiv kt, uint32_t words, int64_t row0) {
     constexpr int LW = word_lanes<FMT>();
     const uint32_t i = (uint32_t)(((uint64_t)blockIdx.x * 256 + threadIdx.x) / LW);
@@ -143,46 +205,53 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
     const uint32_t r = divide(i, kt);
     const int kw = (int)(i - r * kt.d), c = (kw * LW + threadIdx.x % LW) * PER;
     const int64_t row = row0 + r;
-    float v[PER] = {};
+    __shared__ float exchange[8][EXCHANGE];
+    float v[PER];
     const bool live = some && row < o.rows;
-    if (live) load16(static_cast<const uint8_t*>(x) + row * ldx * (dtype == ELT_F32 ? 4 : 2), dtype, vec, c, o.cols, v);
+    load16<LW>(static_cast<const uint8_t*>(x) + row * ldx * (dtype == ELT_F32 ? 4 : 2), dtype, access, c, live ? o.cols : 0,
+               exchange[threadIdx.x / 32], v);
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
     quantize16<FMT>(v, c, row, o.cols, kt.d, o.data, o.ld, o.scales, g, live);
     if (some && !live && threadIdx.x % LW == 0)
         *reinterpret_cast<uint32_t*>(o.scales + mx_scale_word(row, kw, kt.d)) = 0;
 }
 
-// Sixteen elements per thread.
+// Sixteen elements per thread, eight neighbouring threads in one row (`groups`: eights of chunks of a row).
+constexpr int DEQ_GROUP = 8;
 template <int FMT>
-__global__ void __launch_bounds__(256) dequantize_kernel(const __grid_constant__ MxArray x, int kt, FastDiv chunks, uint32_t total,
-                                                         void* out, int dtype, int vec, int64_t ldo, int64_t row0) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-    if (i >= total) return;
-    const uint32_t r = divide(i, chunks);
+__global__ void __launch_bounds__(256) dequantize_kernel(const __grid_constant__ MxArray x, int kt, FastDiv groups, uint32_t total,
+                                                         void* out, int dtype, int access, int64_t ldo, int64_t row0) {
+    __shared__ float exchange[8][EXCHANGE];
+    const uint32_t i = (uint32_t)(((uint64_t)blockIdx.x * 256 + threadIdx.x) / DEQ_GROUP);
+    const uint32_t r = divide(i, groups);
     const int64_t row = row0 + r;
-    const int c = (int)(i - r * chunks.d) * PER;
-    const float g = FMT == NVF4 && x.global_scale ? *x.global_scale : 1.f;
-    const int b = c / mx_block(FMT);
-    const uint32_t code = x.scales[mx_scale_word(row, b / 4, kt) + b % 4];
-    const uint8_t* d = x.data + row * x.ld + mx_bytes(FMT, c);
-    uint32_t u[FMT == MXF8 ? 4 : 2];
-    if constexpr (FMT == MXF8) {
-        const uint4 q = *reinterpret_cast<const uint4*>(d);
-        u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
-    } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(d);
-        u[0] = q.x; u[1] = q.y;
-    }
-    const float s = mx_scale_value<FMT>(code) * g;
-    float v[PER];
+    const int c = ((int)(i - r * groups.d) * DEQ_GROUP + threadIdx.x % DEQ_GROUP) * PER;
+    const bool live = i < total && c < x.cols;
+    float v[PER] = {};
+    if (live) {
+        const float g = FMT == NVF4 && x.global_scale ? *x.global_scale : 1.f;
+        const int b = c / mx_block(FMT);
+        const uint32_t code = x.scales[mx_scale_word(row, b / 4, kt) + b % 4];
+        const uint8_t* d = x.data + row * x.ld + mx_bytes(FMT, c);
+        uint32_t u[FMT == MXF8 ? 4 : 2];
+        if constexpr (FMT == MXF8) {
+            const uint4 q = *reinterpret_cast<const uint4*>(d);
+            u[0] = q.x; u[1] = q.y; u[2] = q.z; u[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(d);
+            u[0] = q.x; u[1] = q.y;
+        }
+        const float s = mx_scale_value<FMT>(code) * g;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t pair = FMT == MXF8 ? u[j / 2] >> (16 * (j % 2)) & 0xffffu : u[j / 4] >> (8 * (j % 4)) & 0xffu;
-        const float2 f = mx_pair_values<FMT>(pair);
-        v[2 * j] = f.x * s;
-        v[2 * j + 1] = f.y * s;
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t pair = FMT == MXF8 ? u[j / 2] >> (16 * (j % 2)) & 0xffffu : u[j / 4] >> (8 * (j % 4)) & 0xffu;
+            const float2 f = mx_pair_values<FMT>(pair);
+            v[2 * j] = f.x * s;
+            v[2 * j + 1] = f.y * s;
+        }
     }
-    store16(static_cast<uint8_t*>(out) + row * ldo * (dtype == ELT_F32 ? 4 : 2), dtype, vec, c, x.cols, v);
+    store16<DEQ_GROUP>(static_cast<uint8_t*>(out) + row * ldo * (dtype == ELT_F32 ? 4 : 2), dtype, access, c, i < total ? x.cols : 0,
+                       exchange[threadIdx.x / 32], v);
 }
 
 struct NormArgs {
@@ -190,9 +259,9 @@ struct NormArgs {
     const void* residual;  // null: the stream is x
     void* residual_out;    // null: not written
     const float* gain;     // null: 1
-    int dtype, res_type, vec, vec_r, vec_ro, vec_g;
+    int dtype, res_type, access, access_r, access_ro, access_g;
     int64_t ldx, ldr, ldro;
-    double eps;
+    double eps, inv_cols;  // inv_cols: 1 / cols
     MxArray o;
     int kt;
     int64_t rows_padded;
@@ -207,6 +276,13 @@ __device__ __forceinline__ void add_squares(uint64_t& sum, uint64_t& err, uint64
     sum = s;
 }
 
+// 1 / sqrt(x) in f64, rounded to f32: the f32 estimate (2 ulp) and one Newton step in f64, which squares its error.
+__device__ __forceinline__ float inverse_root(double x) {
+    if (!(x > 1e-30 && x < 1e30)) return (float)(1.0 / sqrt(x));
+    const double r = rsqrtf((float)x);
+    return (float)fma(0.5 * r, fma(-x * r, r, 1.0), r);
+}
+
 // W warps per row, up to CH chunks of sixteen elements per thread, held in registers: each element is
 // read once. The sum of squares keeps its rounding errors and ends in f64, so 1/rms is the rounded exact one but
 // for rare ties and does not depend on how a row is spread over threads: next to the quantiser's borders its last
@@ -219,19 +295,22 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
     const int t = threadIdx.x % (32 * W), warp = threadIdx.x / 32;
     const bool live = row < a.o.rows;
     const int cols = a.o.cols;
+    __shared__ float exchange[THREADS / 32][EXCHANGE];
+    float* buf = exchange[warp];
     float v[CH][PER];
     float sum = 0.f, err = 0.f;
-    if (live) {
+    {
+        const int n = live ? cols : 0;
         const uint8_t* x = static_cast<const uint8_t*>(a.x) + row * a.ldx * (a.dtype == ELT_F32 ? 4 : 2);
         const uint8_t* r = static_cast<const uint8_t*>(a.residual) + row * a.ldr * (a.res_type == ELT_F32 ? 4 : 2);
         uint8_t* ro = static_cast<uint8_t*>(a.residual_out) + row * a.ldro * (a.res_type == ELT_F32 ? 4 : 2);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) load16(x, a.dtype, a.vec, (t + i * 32 * W) * PER, cols, v[i]);
+        for (int i = 0; i < CH; ++i) load16<32>(x, a.dtype, a.access, (t + i * 32 * W) * PER, n, buf, v[i]);
         if (a.residual) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 float u[PER];
-                load16(r, a.res_type, a.vec_r, (t + i * 32 * W) * PER, cols, u);
+                load16<32>(r, a.res_type, a.access_r, (t + i * 32 * W) * PER, n, buf, u);
 #pragma unroll
                 for (int j = 0; j < PER; j += 2) {
                     f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[j], u[j + 1])), v[i][j], v[i][j + 1]);
@@ -242,7 +321,7 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
         }
         if (a.residual_out) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) store16(ro, a.res_type, a.vec_ro, (t + i * 32 * W) * PER, cols, v[i]);
+            for (int i = 0; i < CH; ++i) store16<32>(ro, a.res_type, a.access_ro, (t + i * 32 * W) * PER, n, buf, v[i]);
         }
         uint64_t s2 = 0, e2 = 0;
 #pragma unroll
@@ -273,7 +352,7 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
 #pragma unroll
         for (int i = 0; i < W; ++i) d += part[warp / W * W + i];
     }
-    const float inv = (float)(1.0 / sqrt(d / cols + a.eps));
+    const float inv = inverse_root(d * a.inv_cols + a.eps);
     const float g = FMT == NVF4 && a.o.global_scale ? *a.o.global_scale : 1.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -281,7 +360,7 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
         if (c - PER * (t % 32) >= cols) break;  // the warp's chunk lies behind the row
         float u[PER];
         if (a.gain) {
-            load16(a.gain, ELT_F32, a.vec_g, c, cols, u);
+            load16<32>(a.gain, ELT_F32, a.access_g, c, cols, buf, u);
         } else {
 #pragma unroll
             for (int j = 0; j < PER; ++j) u[j] = 1.f;
@@ -301,8 +380,9 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
     }
 }
 
-bool rows_aligned(const void* p, int64_t ld, int dtype) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)elt_size(dtype) % 16 == 0;
+int row_access(const void* p, int64_t ld, int dtype) {
+    const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (uint64_t)(ld * (int64_t)elt_size(dtype));
+    return bits % 32 == 0 ? BY_32 : bits % 16 == 0 ? BY_16 : BY_ELEMENT;
 }
 
 template <int FMT, int W, int CH>
@@ -322,7 +402,7 @@ int norm_by_width(const NormArgs& a, cudaStream_t s) {
     if (chunks <= 128) return launch_norm<FMT, 4, 1>(a, s);
     if (chunks <= 256) return launch_norm<FMT, 8, 1>(a, s);
     if (chunks <= 512) return launch_norm<FMT, 8, 2>(a, s);
-    if (chunks <= 2048) return launch_norm<FMT, 32, 2>(a, s);
+    if (chunks <= 2048) return launch_norm<FMT, 16, 4>(a, s);
     return fail(ANCHA_E_UNSUPPORTED, "add_rms_norm: rows wider than 32768");
 }
 
@@ -333,31 +413,31 @@ constexpr int64_t kLaunchItems = int64_t(1) << 30;
 
 int mx_quantize(const void* x, int dtype, int64_t ldx, const MxArray& o, cudaStream_t s) {
     const int64_t kt = mx_ktiles(o.format, o.cols), rows = ceil_div(o.rows, 128) * 128;
-    const int lw = o.format == NVF4 ? word_lanes<NVF4>() : word_lanes<MXF8>(), vec = rows_aligned(x, ldx, dtype);
+    const int lw = o.format == NVF4 ? word_lanes<NVF4>() : word_lanes<MXF8>(), access = row_access(x, ldx, dtype);
     const FastDiv div = fast_div((uint32_t)kt);
     const int64_t step = std::max<int64_t>(1, kLaunchItems / kt);
     for (int64_t r = 0; r < rows; r += step) {
         const uint32_t words = (uint32_t)(std::min(step, rows - r) * kt);
         const unsigned n = (unsigned)ceil_div((int64_t)words * lw, 256);
-        if (o.format == MXF8) quantize_kernel<MXF8><<<n, 256, 0, s>>>(x, dtype, vec, ldx, o, div, words, r);
-        else if (o.format == MXF4) quantize_kernel<MXF4><<<n, 256, 0, s>>>(x, dtype, vec, ldx, o, div, words, r);
-        else quantize_kernel<NVF4><<<n, 256, 0, s>>>(x, dtype, vec, ldx, o, div, words, r);
+        if (o.format == MXF8) quantize_kernel<MXF8><<<n, 256, 0, s>>>(x, dtype, access, ldx, o, div, words, r);
+        else if (o.format == MXF4) quantize_kernel<MXF4><<<n, 256, 0, s>>>(x, dtype, access, ldx, o, div, words, r);
+        else quantize_kernel<NVF4><<<n, 256, 0, s>>>(x, dtype, access, ldx, o, div, words, r);
         ANCHA_TRY(check_launch("mx_quantize"));
     }
     return ANCHA_OK;
 }
 
 int mx_dequantize(const MxArray& x, void* out, int dtype, int64_t ldo, cudaStream_t s) {
-    const int kt = (int)mx_ktiles(x.format, x.cols), vec = rows_aligned(out, ldo, dtype);
-    const int64_t chunks = ceil_div(x.cols, PER);
-    const FastDiv div = fast_div((uint32_t)chunks);
-    const int64_t step = std::max<int64_t>(1, kLaunchItems / chunks);
+    const int kt = (int)mx_ktiles(x.format, x.cols), access = row_access(out, ldo, dtype);
+    const int64_t groups = ceil_div(x.cols, PER * DEQ_GROUP);
+    const FastDiv div = fast_div((uint32_t)groups);
+    const int64_t step = std::max<int64_t>(1, kLaunchItems / groups);
     for (int64_t r = 0; r < x.rows; r += step) {
-        const uint32_t total = (uint32_t)(std::min(step, x.rows - r) * chunks);
-        const unsigned n = (unsigned)ceil_div(total, 256);
-        if (x.format == MXF8) dequantize_kernel<MXF8><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, vec, ldo, r);
-        else if (x.format == MXF4) dequantize_kernel<MXF4><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, vec, ldo, r);
-        else dequantize_kernel<NVF4><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, vec, ldo, r);
+        const uint32_t total = (uint32_t)(std::min(step, x.rows - r) * groups);
+        const unsigned n = (unsigned)ceil_div((int64_t)total * DEQ_GROUP, 256);
+        if (x.format == MXF8) dequantize_kernel<MXF8><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, access, ldo, r);
+        else if (x.format == MXF4) dequantize_kernel<MXF4><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, access, ldo, r);
+        else dequantize_kernel<NVF4><<<n, 256, 0, s>>>(x, kt, div, total, out, dtype, access, ldo, r);
         ANCHA_TRY(check_launch("mx_dequantize"));
     }
     return ANCHA_OK;
@@ -371,10 +451,11 @@ int mx_add_rms_norm(const void* x, int dtype, int64_t ldx, const void* residual,
     a.x = x; a.residual = residual; a.residual_out = residual_out; a.gain = gain;
     a.dtype = dtype; a.res_type = res_type;
     a.ldx = ldx; a.ldr = ldr; a.ldro = ldro;
-    a.vec = rows_aligned(x, ldx, dtype);
-    a.vec_r = residual && rows_aligned(residual, ldr, res_type);
-    a.vec_ro = residual_out && rows_aligned(residual_out, ldro, res_type);
-    a.vec_g = gain && reinterpret_cast<uintptr_t>(gain) % 16 == 0;
+    a.access = row_access(x, ldx, dtype);
+    if (residual) a.access_r = row_access(residual, ldr, res_type);
+    if (residual_out) a.access_ro = row_access(residual_out, ldro, res_type);
+    a.access_g = row_access(gain, 0, ELT_F32);
+    a.inv_cols = 1.0 / o.cols;
     a.eps = eps;
     a.o = o;
     a.kt = (int)mx_ktiles(o.format, o.cols);
