@@ -16,7 +16,7 @@
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace ancha {
 
@@ -172,9 +172,10 @@ __device__ __forceinline__ void mx_encode(const float (&v)[N], const MxBlock& b,
         for (int i = 0; i < W; ++i) {
             float t[8], u[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                t[j] = v[8 * i + j] * lo;
-                u[j] = v[8 * i + j] * hi;
+            for (int j = 0; j < 8; j += 2) {
+                const uint64_t x = f2(v[8 * i + j], v[8 * i + j + 1]);
+                f2_split(fmul2(x, f2(lo, lo)), t[j], t[j + 1]);
+                f2_split(fmul2(x, f2(hi, hi)), u[j], u[j + 1]);
             }
             w[i] = pack_e2m1(t) & mask;
             same = same && w[i] == (pack_e2m1(u) & mask);
@@ -193,7 +194,8 @@ __device__ __forceinline__ void mx_encode(const float (&v)[N], const MxBlock& b,
         for (int i = 0; i < W; ++i) {
             float t[PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j) t[j] = v[PER * i + j] * b.factor;
+            for (int j = 0; j < PER; j += 2)
+                f2_split(fmul2(f2(v[PER * i + j], v[PER * i + j + 1]), f2(b.factor, b.factor)), t[j], t[j + 1]);
             if constexpr (FMT == MXF8) w[i] = pack_e4m3(t[0], t[1], t[2], t[3]) & mask;
             else w[i] = pack_e2m1(t) & mask;
         }

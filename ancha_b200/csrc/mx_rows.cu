@@ -4,7 +4,6 @@
 // block of NVF4, half a block of the others (one shuffle for its maximum), whole 16-byte stores of 8-bit
 // codes, and index arithmetic and scale shared by sixteen.
 #include "mx.cuh"
-#include "tc.cuh"
 
 #include <algorithm>
 
@@ -13,19 +12,43 @@ namespace {
 
 constexpr int PER = 16;  // elements of a row per thread
 
-__device__ __forceinline__ void unpack16(uint32_t u, int type, float& a, float& b) {
-    const float2 f = type == ELT_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u))
-                                      : __half22float2(*reinterpret_cast<const __half2*>(&u));
-    a = f.x;
-    b = f.y;
-}
-__device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
+struct Words8 {
+    uint32_t w[8];
+};
+
+// Sixteen 16-bit elements and their values (the branch on the type is taken once for all).
+__device__ __forceinline__ void unpack16(const Words8& q, int type, float (&v)[PER]) {
     if (type == ELT_BF16) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[2 * j] = __uint_as_float(q.w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(q.w[j] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q.w[j]));
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
     }
-    const __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ Words8 pack16(const float (&v)[PER], int type) {
+    Words8 q;
+    if (type == ELT_BF16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            q.w[j] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            q.w[j] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+    }
+    return q;
 }
 
 __device__ __forceinline__ float element(const void* row, int dtype, int c) {
@@ -37,9 +60,6 @@ __device__ __forceinline__ float element(const void* row, int dtype, int c) {
 // How a row's address allows it to be reached: an element at a time, in 16-byte or in 32-byte pieces.
 enum : int { BY_ELEMENT = 0, BY_16 = 1, BY_32 = 2 };
 
-struct Words8 {
-    uint32_t w[8];
-};
 __device__ __forceinline__ Words8 ld32(const void* p, int access) {
     Words8 q;
     if (access == BY_32) {
@@ -85,9 +105,7 @@ __device__ __forceinline__ void load16(const void* row, int dtype, int access, i
                     for (int j = 0; j < 8; ++j) v[8 * h + j] = __uint_as_float(q.w[j]);
                 }
             } else {
-                const Words8 q = ld32(static_cast<const uint16_t*>(row) + c, access);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) unpack16(q.w[j], dtype, v[2 * j], v[2 * j + 1]);
+                unpack16(ld32(static_cast<const uint16_t*>(row) + c, access), dtype, v);
             }
             return;
         }
@@ -121,9 +139,7 @@ __device__ __forceinline__ void store16(void* row, int dtype, int access, int c,
                     st32(static_cast<float*>(row) + c + 8 * h, access, q);
                 }
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q.w[j] = pack16(v[2 * j], v[2 * j + 1], dtype);
-                st32(static_cast<uint16_t*>(row) + c, access, q);
+                st32(static_cast<uint16_t*>(row) + c, access, pack16(v, dtype));
             }
             return;
         }
@@ -312,16 +328,23 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
                 float u[PER];
                 load16<32>(r, a.res_type, a.access_r, (t + i * 32 * W) * PER, n, buf, u);
 #pragma unroll
-                for (int j = 0; j < PER; j += 2) {
+                for (int j = 0; j < PER; j += 2)
                     f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[j], u[j + 1])), v[i][j], v[i][j + 1]);
-                    // The norm is that of the stream as it is held.
-                    if (a.res_type != ELT_F32) unpack16(pack16(v[i][j], v[i][j + 1], a.res_type), a.res_type, v[i][j], v[i][j + 1]);
-                }
             }
         }
-        if (a.residual_out) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) store16<32>(ro, a.res_type, a.access_ro, (t + i * 32 * W) * PER, n, buf, v[i]);
+        for (int i = 0; i < CH; ++i) {
+            const int c = (t + i * 32 * W) * PER;
+            if (a.res_type != ELT_F32 && a.residual) {
+                // The norm is that of the stream as it is held.
+                const Words8 q = pack16(v[i], a.res_type);
+                unpack16(q, a.res_type, v[i]);
+                if (a.access_ro != BY_ELEMENT && c + PER <= n) {
+                    st32(reinterpret_cast<uint16_t*>(ro) + c, a.access_ro, q);
+                    continue;
+                }
+            }
+            if (a.residual_out) store16<32>(ro, a.res_type, a.access_ro, c, n, buf, v[i]);
         }
         uint64_t s2 = 0, e2 = 0;
 #pragma unroll
