@@ -92,9 +92,10 @@ __device__ __forceinline__ int slot(int e) { return e + (e >> 4); }
 
 // Sixteen elements of a row from column c (a multiple of 16) for every lane, zeros from column `cols` on (cols 0: a lane
 // without a row). GROUP neighbouring lanes hold neighbouring chunks of one row; where its address allows no vector loads
-// they read neighbouring elements together and exchange them through `buf` (a warp's). All lanes of the warp call it.
+// they read neighbouring elements together (fetch16) and then exchange them through `buf`, a warp's (settle16, which all
+// its lanes call): several chunks can be on their way before the first exchange waits for its own.
 template <int GROUP>
-__device__ __forceinline__ void load16(const void* row, int dtype, int access, int c, int cols, float* buf, float (&v)[PER]) {
+__device__ __forceinline__ void fetch16(const void* row, int dtype, int access, int c, int cols, float (&v)[PER]) {
     if (access != BY_ELEMENT) {
         if (c + PER <= cols) {
             if (dtype == ELT_F32) {
@@ -110,16 +111,25 @@ __device__ __forceinline__ void load16(const void* row, int dtype, int access, i
             return;
         }
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = c + j < cols ? element(row, dtype, c + j) : 0.f;
+        for (int j = 0; j < PER; ++j) v[j] = 0.f;
+        if (c < cols) {  // the row's last, shorter chunk
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (c + j < cols) v[j] = element(row, dtype, c + j);
+        }
         return;
     }
-    const int lane = threadIdx.x % 32, sub = lane % GROUP, base = (lane - sub) * PER;
+    const int sub = threadIdx.x % GROUP, first = c - sub * PER + sub;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[k] = first + k * GROUP < cols ? element(row, dtype, first + k * GROUP) : 0.f;
+}
+template <int GROUP>
+__device__ __forceinline__ void settle16(int access, float* buf, float (&v)[PER]) {
+    if (access != BY_ELEMENT) return;
+    const int lane = threadIdx.x % 32, sub = lane % GROUP, base = (lane - sub) * PER + sub;
     __syncwarp();
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int col = c - sub * PER + k * GROUP + sub;
-        buf[slot(base + k * GROUP + sub)] = col < cols ? element(row, dtype, col) : 0.f;
-    }
+    for (int k = 0; k < PER; ++k) buf[slot(base + k * GROUP)] = v[k];
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < PER; ++j) v[j] = buf[slot(lane * PER + j)];
@@ -143,9 +153,11 @@ __device__ __forceinline__ void store16(void* row, int dtype, int access, int c,
             }
             return;
         }
+        if (c < cols) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (c + j < cols) store_elt(row, c + j, v[j], dtype);
+            for (int j = 0; j < PER; ++j)
+                if (c + j < cols) store_elt(row, c + j, v[j], dtype);
+        }
         return;
     }
     const int lane = threadIdx.x % 32, sub = lane % GROUP, base = (lane - sub) * PER;
@@ -224,8 +236,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
     __shared__ float exchange[8][EXCHANGE];
     float v[PER];
     const bool live = some && row < o.rows;
-    load16<LW>(static_cast<const uint8_t*>(x) + row * ldx * (dtype == ELT_F32 ? 4 : 2), dtype, access, c, live ? o.cols : 0,
-               exchange[threadIdx.x / 32], v);
+    fetch16<LW>(static_cast<const uint8_t*>(x) + row * ldx * (dtype == ELT_F32 ? 4 : 2), dtype, access, c, live ? o.cols : 0, v);
+    settle16<LW>(access, exchange[threadIdx.x / 32], v);
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
     quantize16<FMT>(v, c, row, o.cols, kt.d, o.data, o.ld, o.scales, g, live);
     if (some && !live && threadIdx.x % LW == 0)
@@ -304,8 +316,9 @@ __device__ __forceinline__ float inverse_root(double x) {
 // for rare ties and does not depend on how a row is spread over threads: next to the quantiser's borders its last
 // bit decides.
 template <int FMT, int W, int CH>
-__global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(W > 8 ? 32 * W : 256, W > 8 ? 1 : CH > 1 ? 2 : W == 8 ? 6 : W == 1 ? 4 : 5) add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
     constexpr int THREADS = W > 8 ? 32 * W : 256, ROWS = THREADS / (32 * W);
+    constexpr int AHEAD = CH <= 2 ? CH : 1;  // chunks of the residual on their way at once
     __shared__ double part[THREADS / 32];
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / (32 * W);
     const int t = threadIdx.x % (32 * W), warp = threadIdx.x / 32;
@@ -321,16 +334,25 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
         const uint8_t* r = static_cast<const uint8_t*>(a.residual) + row * a.ldr * (a.res_type == ELT_F32 ? 4 : 2);
         uint8_t* ro = static_cast<uint8_t*>(a.residual_out) + row * a.ldro * (a.res_type == ELT_F32 ? 4 : 2);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) load16<32>(x, a.dtype, a.access, (t + i * 32 * W) * PER, n, buf, v[i]);
+        for (int i = 0; i < CH; ++i) fetch16<32>(x, a.dtype, a.access, (t + i * 32 * W) * PER, n, v[i]);
         if (a.residual) {
+            float u[AHEAD][PER];
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                float u[PER];
-                load16<32>(r, a.res_type, a.access_r, (t + i * 32 * W) * PER, n, buf, u);
+                if (i % AHEAD == 0) {
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k)
+                        fetch16<32>(r, a.res_type, a.access_r, (t + (i + k) * 32 * W) * PER, n, u[k]);
+                }
+                settle16<32>(a.access, buf, v[i]);
+                settle16<32>(a.access_r, buf, u[i % AHEAD]);
 #pragma unroll
                 for (int j = 0; j < PER; j += 2)
-                    f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[j], u[j + 1])), v[i][j], v[i][j + 1]);
+                    f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[i % AHEAD][j], u[i % AHEAD][j + 1])), v[i][j], v[i][j + 1]);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) settle16<32>(a.access, buf, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -359,7 +381,7 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
         sum = s;
     }
     double d = (double)sum + (double)err;
-    if (live && !(sum > 1e-30f && sum < 1e37f)) {  // squares near f32's ends (and NaN): in f64
+    if (live && t * PER < cols && !(sum > 1e-30f && sum < 1e37f)) {  // squares near f32's ends (and NaN): in f64
         d = 0.0;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
@@ -383,7 +405,8 @@ __global__ void __launch_bounds__(W > 8 ? 32 * W : 256) add_rms_norm_kernel(cons
         if (c - PER * (t % 32) >= cols) break;  // the warp's chunk lies behind the row
         float u[PER];
         if (a.gain) {
-            load16<32>(a.gain, ELT_F32, a.access_g, c, cols, buf, u);
+            fetch16<32>(a.gain, ELT_F32, a.access_g, c, cols, u);
+            settle16<32>(a.access_g, buf, u);
         } else {
 #pragma unroll
             for (int j = 0; j < PER; ++j) u[j] = 1.f;
@@ -421,10 +444,10 @@ template <int FMT>
 int norm_by_width(const NormArgs& a, cudaStream_t s) {
     const int chunks = (int)ceil_div(a.o.cols, PER);
     if (chunks <= 32) return launch_norm<FMT, 1, 1>(a, s);
-    if (chunks <= 64) return launch_norm<FMT, 1, 2>(a, s);
+    if (chunks <= 64) return launch_norm<FMT, 2, 1>(a, s);
     if (chunks <= 128) return launch_norm<FMT, 4, 1>(a, s);
     if (chunks <= 256) return launch_norm<FMT, 8, 1>(a, s);
-    if (chunks <= 512) return launch_norm<FMT, 8, 2>(a, s);
+    if (chunks <= 512) return launch_norm<FMT, 16, 1>(a, s);
     if (chunks <= 2048) return launch_norm<FMT, 16, 4>(a, s);
     return fail(ANCHA_E_UNSUPPORTED, "add_rms_norm: rows wider than 32768");
 }

@@ -131,10 +131,11 @@ def _matrix(t, device: int, name: str):
         raise _invalid(f"{name}: unsupported dtype {t.dtype}")
     if t.dim() != 2:
         raise _invalid(f"{name}: needs two axes")
-    _on(t, device, name)
+    if t.get_device() != device:
+        raise _invalid(f"{name}: not on the device of the first operand")
+    if t.is_contiguous():  # the stride of a single row is arbitrary in torch
+        return code, t.shape[1] or 1
     rows, cols = t.shape
-    if rows <= 1 and cols <= 1 or t.is_contiguous():  # the stride of a single row is arbitrary in torch
-        return code, max(cols, 1)
     if cols > 1 and t.stride(1) != 1:
         raise _invalid(f"{name}: its last axis must be contiguous")
     return code, (t.stride(0) if rows > 1 else cols)
@@ -185,12 +186,13 @@ def quantize(x: torch.Tensor, format: str = "mxf8", global_scale: Optional[torch
 
 def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``q`` stands for, ``[rows, cols]`` in ``dtype`` (f32, bf16 or f16)."""
-    device = _device(q._data if q._buffer is None else q._buffer)
+    memory = q._data if q._buffer is None else q._buffer
+    device = _device(memory)
     code = _DTYPES.get(dtype)
     if code is None:
         raise _invalid(f"unsupported dtype {dtype}")
     a = _array(q, device, "q")
-    out = torch.empty((q.rows, q.cols), dtype=dtype, device=(q._data if q._buffer is None else q._buffer).device)
+    out = torch.empty_strided((q.rows, q.cols), (q.cols, 1), dtype=dtype, device=memory.device)
     _run(device, N.lib().ancha_mx_dequantize, byref(a), out.data_ptr(), code, q.cols)
     return out
 
@@ -212,7 +214,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, gain:
         res_type, ldr = _matrix(residual, device, "residual")
         res = residual.data_ptr()
         if residual_out is None:
-            residual_out = torch.empty((rows, cols), dtype=residual.dtype, device=x.device)
+            residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
             stream, ldro, res_out = residual_out, cols, residual_out.data_ptr()
     if residual_out is not None and stream is x:
         if residual_out.shape != x.shape or residual_out.dtype != (x if residual is None else residual).dtype:
@@ -257,7 +259,7 @@ def linear(x: Microscaled, weight: Microscaled, bias: Optional[torch.Tensor] = N
     code = _DTYPES.get(dtype)
     if code is None:
         raise _invalid(f"unsupported dtype {dtype}")
-    out = torch.empty((m, n), dtype=dtype, device=memory.device)
+    out = torch.empty_strided((m, n), (n, 1), dtype=dtype, device=memory.device)
     _run(device, N.lib().ancha_mx_linear_fwd, byref(N.MxLinearDesc(ACTIVATIONS[act], code, res_type, n, ldr)), byref(a),
          byref(w), b, res, out.data_ptr(), None)
     return out
