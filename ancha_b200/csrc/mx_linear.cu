@@ -140,17 +140,21 @@ __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32
 // ---- epilogue -------------------------------------------------------------------------------
 
 // GELU(x) = max(x, 0) - |x| Phi(-|x|) with Phi(-u) = 2^R(u), u = min(|x|, 5.5), R a polynomial in
-// v = u 2/5.5 - 1 of degree 9, fitted here to log2 Phi(-u) with the weight u Phi(-u) of the result (Lawson's
-// iteration). Evaluated in f32 its error is f32's: rms 3.9e-8 on [-4, 4], 2.4e-7 at most; the degree 7 fit of
-// the 16-bit epilogues (7e-7) moves the codes of a quantised output more often than the sum's own rounding.
+// v = u 2/5.5 - 1 of degree 7, fitted here to log2 Phi(-u) with the weight u Phi(-u) that its error has in the result
+// (Lawson's iteration). Evaluated in f32 the error is f32's own: rms 5.3e-8 on [-4, 4], 2.5e-7 at most (the
+// 16-bit epilogues' fit of the same degree, weighted for log2 Phi itself, has 7e-7, which moves the codes of a
+// quantised output more often than the product's own rounding). The coefficients lie in constant memory as pairs: as
+// immediates each would cost the packed FMA two moves.
+__constant__ float2 kGelu[8] = {{-8.390578269958496f, -8.390578269958496f}, {-12.107535362243652f, -12.107535362243652f},
+                                {-5.02378511428833f, -5.02378511428833f}, {-0.18455249071121216f, -0.18455249071121216f},
+                                {0.07424018532037735f, 0.07424018532037735f}, {-0.03283032774925232f, -0.03283032774925232f},
+                                {0.015407359227538109f, 0.015407359227538109f}, {0.00019493377476464957f, 0.00019493377476464957f}};
 __device__ __forceinline__ void gelu2(float& x0, float& x1) {
-    constexpr float C[10] = {
-        -8.390586853027344f, -12.107649803161621f, -5.0239338874816895f, -0.18306505680084229f, 0.07878392934799194f,
-        -0.030920876190066338f, 0.009299345314502716f, -0.005405102390795946f, 0.0013578912476077676f, 0.001960539724677801f};
+    const uint64_t* c = reinterpret_cast<const uint64_t*>(kGelu);
     const uint64_t v = ffma2(f2(fminf(fabsf(x0), 5.5f), fminf(fabsf(x1), 5.5f)), f2(2.0f / 5.5f, 2.0f / 5.5f), f2(-1.0f, -1.0f));
-    uint64_t r = f2(C[9], C[9]);
+    uint64_t r = c[7];
 #pragma unroll
-    for (int i = 8; i >= 0; --i) r = ffma2(r, v, f2(C[i], C[i]));
+    for (int i = 6; i >= 0; --i) r = ffma2(r, v, c[i]);
     float r0, r1;
     f2_split(r, r0, r1);
     x0 = fmaf(-fabsf(x0), ex2_approx(r0), fmaxf(x0, 0.f));
@@ -303,11 +307,10 @@ __device__ __forceinline__ void store_plain(const Params& p, float* buf, int64_t
         store_elt(p.out, (row0 + r) * p.ldo + c0 + lane, buf[r * 32 + (lane ^ r)], p.out_type);
 }
 
-// A lane's 32 columns quantised: one block of 32, or two of 16, in its registers. All lanes of the warp call it,
-// lane l for row row0 + l; rows from m on are not written.
-// Returns the scale code, or the two.
+// A lane's 32 columns quantised, one block of 32 or two of 16, in its registers; the codes go to its row of the staging
+// buffer (half `half` of 64 columns). Returns the scale code, or the two.
 template <int FMT>
-__device__ __forceinline__ uint32_t store_mx(const MxArray& o, int64_t row0, int m, int c0, int lane, const float (&v)[32]) {
+__device__ __forceinline__ uint32_t stage_mx(const MxArray& o, uint8_t* buf, int half, int lane, const float (&v)[32]) {
     constexpr int B = mx_block(FMT), W = FMT == MXF8 ? 8 : 4;
     const float g = FMT == NVF4 && o.global_scale ? *o.global_scale : 1.f;
     uint32_t codes = 0, w[W];
@@ -325,31 +328,20 @@ __device__ __forceinline__ uint32_t store_mx(const MxArray& o, int64_t row0, int
 #pragma unroll
         for (int j = 0; j < W * B / 32; ++j) w[h * (W * B / 32) + j] = e[j];
     }
-    const int64_t row = row0 + lane;
+    // Rows of 64 bytes with the 64-byte swizzle (mxf8), of 32 with the 32-byte swizzle.
     if (FMT == MXF8) {
-        // Two lanes write a row's 32 bytes together, so that a store covers whole sectors: the even lane's row first,
-        // then the odd one's.
-        const bool odd = lane & 1;
-        uint4 own = make_uint4(w[0], w[1], w[2], w[3]), peer;
-        const uint4 hi = make_uint4(w[4 % W], w[5 % W], w[6 % W], w[7 % W]);
-        peer.x = __shfl_xor_sync(0xffffffffu, odd ? own.x : hi.x, 1);
-        peer.y = __shfl_xor_sync(0xffffffffu, odd ? own.y : hi.y, 1);
-        peer.z = __shfl_xor_sync(0xffffffffu, odd ? own.z : hi.z, 1);
-        peer.w = __shfl_xor_sync(0xffffffffu, odd ? own.w : hi.w, 1);
-        const int64_t even_row = row - odd;
-        uint8_t* d = o.data + even_row * o.ld + c0 + 16 * odd;
-        if (c0 + 16 * odd < o.cols) {
-            if (even_row < m) *reinterpret_cast<uint4*>(d) = odd ? peer : own;
-            if (even_row + 1 < m) *reinterpret_cast<uint4*>(d + o.ld) = odd ? hi : peer;
-        }
-    } else if (row < m) {
-        *reinterpret_cast<uint4*>(o.data + row * o.ld + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        buf += lane * 64;
+        *reinterpret_cast<uint4*>(buf + ((2 * half) ^ ((lane >> 1) & 3)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(buf + ((2 * half + 1) ^ ((lane >> 1) & 3)) * 16) = make_uint4(w[4 % W], w[5 % W], w[6 % W], w[7 % W]);
+    } else {
+        *reinterpret_cast<uint4*>(buf + lane * 32 + (half ^ ((lane >> 2) & 1)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return codes;
 }
 
 // A converged warp's wait; false where one lane's ran out.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;  // no clock read where there is no wait
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err));
 }
 
@@ -489,45 +481,46 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
         float* bias = reinterpret_cast<float*>(staging + EPI * STAGING) + (warp - 2) * 64;
         float alpha = 1.f;
         if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
-        const bool wide = p.out_type == ELT_F32;
+        const bool wide = p.out_mode == OUT_TMA && p.out_type == ELT_F32;
+        float b0 = 0.f, b1 = 0.f;
+        const auto load_bias = [&](int t) {
+            const int c = t % p.n_tiles * BN + col0 + lane;
+            b0 = c < p.n ? p.bias[c] : 0.f;
+            b1 = c + 32 < p.n ? p.bias[c + 32] : 0.f;
+        };
+        if (p.bias && tile0 < p.tiles) load_bias(tile0);
         uint32_t local = 0;
         for (int t = tile0; t < p.tiles; t += tstep, ++local) {
             const int m0 = t / p.n_tiles * BMT, c_first = t % p.n_tiles * BN + col0;
             const int b = local & 1;
-            // The tile's bias, on its way while the products run: read in the epilogue it would cost each chunk the
-            // latency of L2.
-            float b0 = 0.f, b1 = 0.f;
-            if (p.bias) {
-                if (c_first + lane < p.n) b0 = p.bias[c_first + lane];
-                if (c_first + 32 + lane < p.n) b1 = p.bias[c_first + 32 + lane];
-            }
+            // The tile's bias, on its way since the tile before: read when it is needed it would cost the latency of L2.
             __syncwarp();
             bias[lane] = b0;
             bias[32 + lane] = b1;
+            if (p.bias && t + tstep < p.tiles) load_bias(t + tstep);
             if (!warp_wait(&tfull[b], (local >> 1) & 1, abort, p.err)) break;
             tc_fence_after();
             const int64_t row0 = m0 + (int)rank * BM + quarter * 32, row = row0 + lane;
             const bool some = row0 < p.m && c_first < p.n;
             const uint32_t base = tmem + b * S::ACC1 + col0 + ((uint32_t)(quarter * 32) << 16);
-            uint32_t codes = 0;
-#pragma unroll 1
+            uint32_t codes = 0, r[2][32];
+            tmem_ld32(base, r[0]);
+            tmem_ld32(base + 32, r[1]);
+            tmem_wait_ld();
+            // This warp is done with the accumulator (and with every earlier one).
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
+                if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0));
+                else mbar_arrive(bar);
+            }
+#pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t r[32];
-                tmem_ld32(base + 32 * h, r);
-                tmem_wait_ld();
-                if (h == 1) {  // this warp is done with the accumulator (and with every earlier one)
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
-                        if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0));
-                        else mbar_arrive(bar);
-                    }
-                }
                 const int c0 = c_first + 32 * h, nv = min(32, p.n - c0);
                 if (nv <= 0 || !some) continue;
                 float v[32];
-                finish32<FMT == NVF4>(p, bias + 32 * h, row, row < p.m, c0, nv, alpha, r, v);
+                finish32<FMT == NVF4>(p, bias + 32 * h, row, row < p.m, c0, nv, alpha, r[h], v);
                 if (p.out_mode == OUT_TMA) {
                     if (wide || h == 0) {  // the store that last read the buffer is done with it
                         if (elect_one()) bulk_wait_read<0>();
@@ -544,19 +537,21 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     }
                 } else if (p.out_mode == OUT_PLAIN) {
                     store_plain(p, reinterpret_cast<float*>(stage), row0, c0, nv, lane, v);
-                } else if (p.om.format == MXF8) {
-                    codes |= store_mx<MXF8>(p.om, row0, p.m, c0, lane, v) << (8 * h);
-                } else if (p.om.format == MXF4) {
-                    codes |= store_mx<MXF4>(p.om, row0, p.m, c0, lane, v) << (8 * h);
                 } else {
-                    codes |= store_mx<NVF4>(p.om, row0, p.m, c0, lane, v) << (16 * h);
+                    if (h == 0) {
+                        if (elect_one()) bulk_wait_read<0>();
+                        __syncwarp();
+                    }
+                    if (p.om.format == MXF8) codes |= stage_mx<MXF8>(p.om, stage, h, lane, v) << (8 * h);
+                    else if (p.om.format == MXF4) codes |= stage_mx<MXF4>(p.om, stage, h, lane, v) << (8 * h);
+                    else codes |= stage_mx<NVF4>(p.om, stage, h, lane, v) << (16 * h);
                 }
             }
-            if (p.out_mode == OUT_TMA && !wide && some) {
+            if (p.out_mode != OUT_PLAIN && !wide && some) {
                 fence_proxy_async();
                 __syncwarp();
                 if (elect_one()) {
-                    tma_store_3d(&tout, stage, c_first, (int)row0, 0);
+                    tma_store_3d(&tout, stage, p.out_mode == OUT_MX && p.om.format != MXF8 ? c_first / 2 : c_first, (int)row0, 0);
                     bulk_commit();
                 }
             }
@@ -803,8 +798,8 @@ int launch_split(const MxLinear& q, const Params& p, int splits, cudaStream_t s)
     }
     CUtensorMap tw, tx, tsw, tsx;
     const int64_t kt = mx_ktiles(FMT, q.x.cols);
-    ANCHA_TRY(make_tma_bytes(&tw, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, BM, true));
-    ANCHA_TRY(make_tma_bytes(&tx, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, TN, true));
+    ANCHA_TRY(make_tma_bytes(&tw, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, BM, 128));
+    ANCHA_TRY(make_tma_bytes(&tx, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, TN, 128));
     ANCHA_TRY(make_tma_scales(&tsw, q.w.scales, kt, ceil_div(p.n, 128), S::SF, 1));
     ANCHA_TRY(make_tma_scales(&tsx, q.x.scales, kt, ceil_div(p.m, 128), S::SF, 1));
     cudaLaunchAttribute attr[1];
@@ -854,12 +849,15 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     }
     CUtensorMap ta, tb, tsa, tsb, to;
     const int64_t akt = mx_ktiles(FMT, q.x.cols);
-    ANCHA_TRY(make_tma_bytes(&ta, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, BM, true));
-    ANCHA_TRY(make_tma_bytes(&tb, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, S::B_ROWS, true));
+    ANCHA_TRY(make_tma_bytes(&ta, q.x.data, p.kbytes, p.m, q.x.ld, SLAB, BM, 128));
+    ANCHA_TRY(make_tma_bytes(&tb, q.w.data, p.kbytes, p.n, q.w.ld, SLAB, S::B_ROWS, 128));
     ANCHA_TRY(make_tma_scales(&tsa, q.x.scales, akt, ceil_div(p.m, 128), S::SF, 1));
     ANCHA_TRY(make_tma_scales(&tsb, q.w.scales, akt, ceil_div(p.n, 128), S::SF, S::RANGES));
     to = ta;
-    if (p.out_mode == OUT_TMA)
+    if (p.out_mode == OUT_MX)
+        ANCHA_TRY(make_tma_bytes(&to, p.om.data, mx_row_bytes(p.om.format, p.om.cols), p.m, p.om.ld,
+                                 p.om.format == MXF8 ? 64 : 32, 32, p.om.format == MXF8 ? 64 : 32));
+    else if (p.out_mode == OUT_TMA)
         ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, p.out_type == ELT_F32 ? 32 : 64, 32));
     p.m_tiles = (int)ceil_div(p.m, PAIR ? 2 * BM : BM);
     p.n_tiles = (int)ceil_div(p.n, BN);

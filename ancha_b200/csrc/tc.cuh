@@ -46,9 +46,9 @@ int make_tma_store_3d(CUtensorMap* map, const void* base, int elt, int64_t cols,
                       int64_t depth, int64_t ld, int64_t depth_stride, int box_cols, int box_rows);
 
 // Encode a tiled tensor map over `rows` rows of `row_bytes` bytes, `ld` bytes apart, with a {box_bytes,
-// box_rows, 1} box; `swizzle`: 128-byte swizzle (box_bytes 128). Zero fill out of bounds.
+// box_rows, 1} box; `swizzle`: 128, 64 or 32 bytes, box_bytes the same. Zero fill out of bounds.
 int make_tma_bytes(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int64_t ld, int box_bytes,
-                   int box_rows, bool swizzle);
+                   int box_rows, int swizzle);
 
 // Encode a tensor map over the scale tiles of a microscaled array (`mt` row ranges of `kt` tiles of 512
 // bytes, as 256-byte rows) with a box of `box_k` tiles along a row by `box_m` row ranges: coordinates

@@ -149,7 +149,7 @@ int make_tma_4d(CUtensorMap* map, const void* base, int elt, int64_t cols, int64
 }
 
 int make_tma_bytes(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows, int64_t ld, int box_bytes,
-                   int box_rows, bool swizzle) {
+                   int box_rows, int swizzle) {
     auto fn = encode_fn();
     if (!fn) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
     if (reinterpret_cast<uintptr_t>(base) % 16 || ld % 16 || row_bytes <= 0 || rows <= 0)
@@ -159,7 +159,9 @@ int make_tma_bytes(CUtensorMap* map, const void* base, int64_t row_bytes, int64_
     const cuuint32_t box[3] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                                     : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                                     : CU_TENSOR_MAP_SWIZZLE_32B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(ANCHA_E_UNSUPPORTED, "cuTensorMapEncodeTiled (bytes) failed: " + std::to_string((int)r));
     return ANCHA_OK;
