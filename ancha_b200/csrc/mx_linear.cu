@@ -39,8 +39,16 @@ struct Shape {
     static constexpr int STAGE = OPERAND_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
     static constexpr int EPI = BN / 16;                 // epilogue warps: 32 rows by 64 columns of the tile each
     static constexpr int THREADS = 64 + 32 * EPI;
-    static constexpr int FIT = (227 * 1024 - 1024 - 256 - EPI * (STAGING + BIAS_BYTES)) / STAGE, STAGES = FIT < 6 ? FIT : 6;
-    static constexpr int BYTES = 1024 + STAGES * STAGE + EPI * (STAGING + BIAS_BYTES) + 256;
+    // Stages and bytes of shared memory; with a residual that TMA can read each epilogue warp has a second buffer.
+    static constexpr int FIXED = 1024 + 512 + EPI * (STAGING + BIAS_BYTES);
+    static constexpr int stages(bool residual) {
+        const int fit = (227 * 1024 - FIXED - (residual ? EPI * STAGING : 0)) / STAGE;
+        return fit < 6 ? fit : 6;
+    }
+    static constexpr int bytes(bool residual) {
+        return FIXED + (residual ? EPI * STAGING : 0) + stages(residual) * STAGE;
+    }
+    static_assert(stages(true) >= 2, "shared memory");
     // Second accumulator. Two of 256 columns and the scales do not fit 512: they share 64 columns, which
     // the epilogue of a tile drains first, so the next tile's products start when those are free.
     static constexpr uint32_t ACC1 = BN == 256 ? 192 : BN;
@@ -55,14 +63,18 @@ struct Params {
     const float* bias;
     const void* residual;
     int64_t ldr;
-    int res_type, res_vec, act;
+    int res_type, res_mode, act;  // res_mode: RES_*
     void* out;
     int64_t ldo;
     int out_type, out_mode;    // OUT_*
     MxArray om;
     int okt;                   // scale tiles along a row of om
+    int oblock_log2;           // its block
+    int rows_padded;           // m rounded to whole scale tiles
+    int stages;
     int* err;
 };
+enum : int { RES_NONE = 0, RES_ELEMENT = 1, RES_TMA = 2 };  // RES_TMA: 16-byte aligned rows
 enum : int { OUT_TMA = 0, OUT_PLAIN = 1, OUT_MX = 2 };
 
 // ---- block-scaled tcgen05 -------------------------------------------------------------------
@@ -167,12 +179,29 @@ __device__ __forceinline__ float residual_at(const Params& p, int64_t i) {
                                     : __half2float(static_cast<const __half*>(p.residual)[i]);
 }
 
+// v[j ..] += four f32, or eight elements of 16 bits.
+__device__ __forceinline__ void add4(const float4& q, float (&v)[32], int j) {
+    f2_split(fadd2(f2(v[j], v[j + 1]), f2(q.x, q.y)), v[j], v[j + 1]);
+    f2_split(fadd2(f2(v[j + 2], v[j + 3]), f2(q.z, q.w)), v[j + 2], v[j + 3]);
+}
+__device__ __forceinline__ void add8(const uint4& q, int type, float (&v)[32], int j) {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = type == ELT_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]))
+                                          : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[j + 2 * i] += f.x;
+        v[j + 2 * i + 1] += f.y;
+    }
+}
+
 // act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them); `bias`: theirs, in shared
-// memory. The arithmetic
+// memory, as with RES `res`, the rows of the residual (32 columns of f32, or 64 of 16 bits of which half `half`). The
+// arithmetic
 // runs on packed pairs, one instruction for two values: the epilogue is bound by instruction issue.
-template <bool SCALED>
-__device__ __forceinline__ void finish32(const Params& p, const float* bias, int64_t row, bool live, int c0, int nv,
-                                         float alpha, const uint32_t (&r)[32], float (&v)[32]) {
+template <bool SCALED, bool RES>
+__device__ __forceinline__ void finish32(const Params& p, const float* bias, const uint8_t* res, int half, int lane, int64_t row,
+                                         bool live, int c0, int nv, float alpha, const uint32_t (&r)[32], float (&v)[32]) {
     const uint64_t al = f2(alpha, alpha);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
@@ -189,36 +218,20 @@ __device__ __forceinline__ void finish32(const Params& p, const float* bias, int
 #pragma unroll
         for (int j = 0; j < 32; j += 2) tanh_fast2(v[j], v[j + 1]);
     }
-    if (p.residual && live) {
-        const int64_t at = row * p.ldr + c0;
-        if (p.res_vec && nv == 32) {
-            if (p.res_type == ELT_F32) {
+    if (RES) {
+        if (p.res_type == ELT_F32) {
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at + j);
-                    f2_split(fadd2(f2(v[j], v[j + 1]), f2(q.x, q.y)), v[j], v[j + 1]);
-                    f2_split(fadd2(f2(v[j + 2], v[j + 3]), f2(q.z, q.w)), v[j + 2], v[j + 3]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at + j);
-                    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = p.res_type == ELT_BF16
-                                             ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]))
-                                             : __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-                        v[j + 2 * i] += f.x;
-                        v[j + 2 * i + 1] += f.y;
-                    }
-                }
-            }
+            for (int q = 0; q < 8; ++q)
+                add4(*reinterpret_cast<const float4*>(res + lane * 128 + ((q ^ (lane & 7)) * 16)), v, 4 * q);
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (j < nv) v[j] += residual_at(p, at + j);
+            for (int q = 0; q < 4; ++q)
+                add8(*reinterpret_cast<const uint4*>(res + lane * 128 + (((q + 4 * half) ^ (lane & 7)) * 16)), p.res_type, v, 8 * q);
         }
+    } else if (p.res_mode != RES_NONE && live) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < nv) v[j] += residual_at(p, row * p.ldr + c0 + j);
     }
     if (nv < 32) {
 #pragma unroll
@@ -345,25 +358,47 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err));
 }
 
-template <int FMT, int BN, bool PAIR>
+// The tiles of a CTA (or pair), tile0, tile0 + step, ..., as row and column of the tile grid: divided once.
+struct TileWalk {
+    int mi, ni, dm, dn, n_tiles;
+    __device__ __forceinline__ TileWalk(int tile0, int step, int n) : n_tiles(n) {
+        mi = tile0 / n; ni = tile0 - mi * n;
+        dm = step / n; dn = step - dm * n;
+    }
+    __device__ __forceinline__ void next() {
+        mi += dm;
+        ni += dn;
+        if (ni >= n_tiles) {
+            ni -= n_tiles;
+            ++mi;
+        }
+    }
+};
+
+template <int FMT, int BN, bool PAIR, bool RES>
 __global__ void __launch_bounds__(Shape<FMT, BN, PAIR>::THREADS, 1)
 linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
               const __grid_constant__ CUtensorMap tsa, const __grid_constant__ CUtensorMap tsb,
-              const __grid_constant__ CUtensorMap tout, const __grid_constant__ Params p) {
+              const __grid_constant__ CUtensorMap tout, const __grid_constant__ CUtensorMap tres,
+              const __grid_constant__ Params p) {
     using S = Shape<FMT, BN, PAIR>;
-    constexpr int BMT = PAIR ? 2 * BM : BM, STAGES = S::STAGES, EPI = S::EPI;
+    constexpr int BMT = PAIR ? 2 * BM : BM, EPI = S::EPI;
+    const int stages = p.stages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* a_tiles = smem;
-    uint8_t* b_tiles = a_tiles + STAGES * OPERAND_BYTES;
-    uint8_t* staging = b_tiles + STAGES * S::B_BYTES;  // 1024-byte aligned, as the operands
-    uint8_t* sa_tiles = staging + EPI * (STAGING + BIAS_BYTES);
-    uint8_t* sb_tiles = sa_tiles + STAGES * S::SFA_BYTES;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + STAGES * S::SFB_BYTES);
-    uint64_t* empty = full + STAGES;
-    uint64_t* tfull = empty + STAGES;   // [2] accumulator ready
+    uint8_t* b_tiles = a_tiles + stages * OPERAND_BYTES;
+    uint8_t* staging = b_tiles + stages * S::B_BYTES;  // 1024-byte aligned, as the operands
+    uint8_t* residual = staging + EPI * STAGING;  // with RES
+    uint8_t* biases = residual + (RES ? EPI * STAGING : 0);
+    uint8_t* sa_tiles = biases + EPI * BIAS_BYTES;
+    uint8_t* sb_tiles = sa_tiles + stages * S::SFA_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + stages * S::SFB_BYTES);
+    uint64_t* empty = full + stages;
+    uint64_t* tfull = empty + stages;   // [2] accumulator ready
     uint64_t* tempty = tfull + 2;       // [2] accumulator drained (with shared columns: [0], those drained)
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    uint64_t* rfull = tempty + 2;       // [EPI] residual arrived
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + EPI);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -371,7 +406,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     const int tile0 = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x;
     const int tstep = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -379,6 +414,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             mbar_init(&tfull[b], 1);
             mbar_init(&tempty[b], PAIR ? 2 * EPI : EPI);
         }
+        for (int w = 0; w < EPI; ++w) mbar_init(&rfull[w], 1);
         *abort = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -402,14 +438,15 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int slabs = (p.kbytes + SLAB - 1) / SLAB;
+    TileWalk walk(tile0, tstep, p.n_tiles);
 
     if (warp == 0) {
-        uint32_t it = 0;
-        for (int t = tile0; t < p.tiles && !*abort; t += tstep) {
-            const int m0 = t / p.n_tiles * BMT, n0 = t % p.n_tiles * BN;
+        int s = 0;
+        uint32_t it = 0, phase = 1;
+        for (int t = tile0; t < p.tiles && !*abort; t += tstep, walk.next()) {
+            const int m0 = walk.mi * BMT, n0 = walk.ni * BN;
             for (int kb = 0; kb < slabs; ++kb, ++it) {
-                const int s = it % STAGES;
-                if (!warp_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort, p.err)) break;
+                if (!warp_wait(&empty[s], phase, abort, p.err)) break;
                 if (elect_one()) {
                     uint8_t* a = a_tiles + s * OPERAND_BYTES;
                     uint8_t* b = b_tiles + s * S::B_BYTES;
@@ -432,20 +469,25 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     }
                 }
                 __syncwarp();
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
         }
         if (*abort && rank == 0 && lane == 0) {  // let copies in flight land before the CTA exits (bounded)
             const long long c0 = clock64();
-            for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
-                while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
+            for (uint32_t j = it > (uint32_t)stages ? it - stages : 0; j < it; ++j)
+                while (!mbar_try_wait(&full[j % stages], (j / stages) & 1) && clock64() - c0 < kWaitCycles) {
                 }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
             constexpr uint32_t idesc = idesc_of<FMT>(BMT, BN);
-            uint32_t it = 0, local = 0;
-            for (int t = tile0; t < p.tiles && !*abort; t += tstep, ++local) {
+            int s = 0;
+            uint32_t phase = 0, local = 0;
+            for (int t = tile0; t < p.tiles && !*abort; t += tstep, ++local, walk.next()) {
                 const int b = local & 1;
                 if (S::SHARED_COLS) {
                     if (local && !warp_wait(&tempty[0], (local - 1) & 1, abort, p.err)) break;
@@ -454,16 +496,15 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 }
                 tc_fence_after();
                 const uint32_t acc = tmem + b * S::ACC1;
-                for (int kb = 0; kb < slabs; ++kb, ++it) {
-                    const int s = it % STAGES;
-                    if (!warp_wait(&full[s], (it / STAGES) & 1, abort, p.err)) break;
+                for (int kb = 0; kb < slabs; ++kb) {
+                    if (!warp_wait(&full[s], phase, abort, p.err)) break;
                     tc_fence_after();
                     const int steps = min(4, (p.kbytes - kb * SLAB + 31) / 32);
                     if (elect_one()) {
                         slab_products<FMT, PAIR, BN>(acc, tmem + SFA_COL, tmem + SFB_COL, smem_u32(a_tiles + s * OPERAND_BYTES),
                                                      smem_u32(b_tiles + s * S::B_BYTES), smem_u32(sa_tiles + s * S::SFA_BYTES),
                                                      smem_u32(sb_tiles + s * S::SFB_BYTES), idesc, steps, kb == 0,
-                                                     BN == 192 ? (uint32_t)(t % p.n_tiles & 1) * 2 : 0);
+                                                     BN == 192 ? (uint32_t)(walk.ni & 1) * 2 : 0);
                         if (PAIR) umma_commit_pair(&empty[s], 0x3);
                         else umma_commit(&empty[s]);
                         if (kb == slabs - 1) {
@@ -472,37 +513,57 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                         }
                     }
                     __syncwarp();
+                    if (++s == stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
     } else {
         const int quarter = warp % 4, col0 = (warp - 2) / 4 * 64;
         uint8_t* stage = staging + (warp - 2) * STAGING;
-        float* bias = reinterpret_cast<float*>(staging + EPI * STAGING) + (warp - 2) * 64;
+        uint8_t* res = residual + (warp - 2) * STAGING;
+        uint64_t* rbar = &rfull[warp - 2];
+        float* bias = reinterpret_cast<float*>(biases) + (warp - 2) * 64;
         float alpha = 1.f;
         if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
         const bool wide = p.out_mode == OUT_TMA && p.out_type == ELT_F32;
         float b0 = 0.f, b1 = 0.f;
-        const auto load_bias = [&](int t) {
-            const int c = t % p.n_tiles * BN + col0 + lane;
+        const auto load_bias = [&](int ni) {
+            const int c = ni * BN + col0 + lane;
             b0 = c < p.n ? p.bias[c] : 0.f;
             b1 = c + 32 < p.n ? p.bias[c + 32] : 0.f;
         };
-        if (p.bias && tile0 < p.tiles) load_bias(tile0);
+        if (p.bias && tile0 < p.tiles) load_bias(walk.ni);
+        // The residual's 32 x 32 f32, or 32 x 64 elements of 16 bits, in the layout of the staging buffer.
+        const bool res_wide = p.res_type == ELT_F32;
+        uint32_t res_phase = 0;
+        bool res_pending = false;
+        const auto load_res = [&](int c, int64_t row0) {
+            __syncwarp();  // every lane has read the buffer
+            if (elect_one()) {
+                mbar_arrive_expect_tx(rbar, STAGING);
+                tma_load_3d(res, &tres, rbar, c, (int)row0, 0);
+            }
+            res_pending = true;
+        };
         uint32_t local = 0;
         for (int t = tile0; t < p.tiles; t += tstep, ++local) {
-            const int m0 = t / p.n_tiles * BMT, c_first = t % p.n_tiles * BN + col0;
-            const int b = local & 1;
+            const int c_first = walk.ni * BN + col0, b = local & 1;
+            const int64_t row0 = (int64_t)walk.mi * BMT + (int)rank * BM + quarter * 32, row = row0 + lane;
+            const bool some = row0 < p.m && c_first < p.n;
+            walk.next();
             // The tile's bias, on its way since the tile before: read when it is needed it would cost the latency of L2.
             __syncwarp();
             bias[lane] = b0;
             bias[32 + lane] = b1;
-            if (p.bias && t + tstep < p.tiles) load_bias(t + tstep);
+            if (p.bias && t + tstep < p.tiles) load_bias(walk.ni);
+            if (RES && some) load_res(c_first, row0);
             if (!warp_wait(&tfull[b], (local >> 1) & 1, abort, p.err)) break;
             tc_fence_after();
-            const int64_t row0 = m0 + (int)rank * BM + quarter * 32, row = row0 + lane;
-            const bool some = row0 < p.m && c_first < p.n;
             const uint32_t base = tmem + b * S::ACC1 + col0 + ((uint32_t)(quarter * 32) << 16);
+            bool res_ok = true;
             uint32_t codes = 0, r[2][32];
             tmem_ld32(base, r[0]);
             tmem_ld32(base + 32, r[1]);
@@ -520,7 +581,14 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 const int c0 = c_first + 32 * h, nv = min(32, p.n - c0);
                 if (nv <= 0 || !some) continue;
                 float v[32];
-                finish32<FMT == NVF4>(p, bias + 32 * h, row, row < p.m, c0, nv, alpha, r[h], v);
+                if (RES && res_pending) {
+                    res_ok = warp_wait(rbar, res_phase, abort, p.err);
+                    if (!res_ok) break;
+                    res_phase ^= 1;
+                    res_pending = false;
+                }
+                finish32<FMT == NVF4, RES>(p, bias + 32 * h, res, h, lane, row, row < p.m, c0, nv, alpha, r[h], v);
+                if (RES && res_wide && h == 0 && c0 + 32 < p.n) load_res(c0 + 32, row0);
                 if (p.out_mode == OUT_TMA) {
                     if (wide || h == 0) {  // the store that last read the buffer is done with it
                         if (elect_one()) bulk_wait_read<0>();
@@ -547,6 +615,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                     else codes |= stage_mx<NVF4>(p.om, stage, h, lane, v) << (16 * h);
                 }
             }
+            if (RES && !res_ok) break;
             if (p.out_mode != OUT_PLAIN && !wide && some) {
                 fence_proxy_async();
                 __syncwarp();
@@ -557,15 +626,21 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             }
             if (p.out_mode == OUT_MX) {
                 // The scales of 64 columns; 0 behind the last row and column, as far as the scale tiles reach.
-                const int block = mx_block(p.om.format), blk = c_first / block;
-                if (row < ((int64_t)p.m + 127) / 128 * 128 && blk / 4 < p.okt) {
+                const int blk = c_first >> p.oblock_log2;
+                if (row < p.rows_padded && blk / 4 < p.okt) {
                     uint8_t* sc = p.om.scales + mx_scale_word(row, blk / 4, p.okt) + blk % 4;
                     if (row >= p.m) codes = 0;
-                    if (block == 32) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)codes;
+                    if (p.oblock_log2 == 5) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)codes;
                     else *reinterpret_cast<uint32_t*>(sc) = codes;
                 }
             }
         }
+        if (RES && res_pending && lane == 0) {  // after an abort: the copy in flight lands before the CTA exits (bounded)
+            const long long c0 = clock64();
+            while (!mbar_try_wait(rbar, res_phase) && clock64() - c0 < kWaitCycles) {
+            }
+        }
+        __syncwarp();
         if (elect_one()) bulk_wait<0>();
         __syncwarp();
     }
@@ -750,7 +825,7 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
     for (int c = rank + warp * splits; c < live; c += SPLIT_WARPS * splits) {
         const int64_t row = m0 + c;
         float res[4] = {};
-        if (p.residual) load4(p.residual, p.res_type, p.res_vec, row * p.ldr + col, nv, res);
+        if (p.residual) load4(p.residual, p.res_type, p.res_mode == RES_TMA, row * p.ldr + col, nv, res);
         float v[4] = {};
         const uint32_t at = smem_u32(partial + c * BM + 4 * lane);
         for (int k = 0; k < splits; ++k) {
@@ -818,10 +893,11 @@ int launch_split(const MxLinear& q, const Params& p, int splits, cudaStream_t s)
     return check_launch("mx_linear (split)");
 }
 
-template <int FMT, int BN, bool PAIR>
+// RES: a residual that TMA can read (the kernel without it keeps its registers).
+template <int FMT, int BN, bool PAIR, bool RES>
 int launch(const MxLinear& q, Params p, cudaStream_t s) {
     using S = Shape<FMT, BN, PAIR>;
-    auto kernel = linear_kernel<FMT, BN, PAIR>;
+    auto kernel = linear_kernel<FMT, BN, PAIR, RES>;
     static int slots[64] = {};  // co-resident CTAs (one per SM) or CTA pairs
     int dev = 0;
     ANCHA_CUDA(cudaGetDevice(&dev));
@@ -832,11 +908,12 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(S::THREADS, 1, 1);
-    cfg.dynamicSmemBytes = S::BYTES;
+    p.stages = S::stages(RES);
+    cfg.dynamicSmemBytes = S::bytes(RES);
     cfg.attrs = attr;
     cfg.numAttrs = PAIR ? 1 : 0;
     if (!slots[dev & 63]) {
-        ANCHA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+        ANCHA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(RES)));
         int n = 0;
         if (PAIR) {
             cfg.gridDim = dim3(2, 1, 1);
@@ -859,6 +936,10 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
                                  p.om.format == MXF8 ? 64 : 32, 32, p.om.format == MXF8 ? 64 : 32));
     else if (p.out_mode == OUT_TMA)
         ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, p.out_type == ELT_F32 ? 32 : 64, 32));
+    CUtensorMap tr = ta;
+    if (RES)
+        ANCHA_TRY(make_tma_store_3d(&tr, p.residual, p.res_type, p.n, p.m, 1, p.ldr, (int64_t)p.m * p.ldr,
+                                    p.res_type == ELT_F32 ? 32 : 64, 32));
     p.m_tiles = (int)ceil_div(p.m, PAIR ? 2 * BM : BM);
     p.n_tiles = (int)ceil_div(p.n, BN);
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
@@ -867,14 +948,19 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     const int units = std::min(p.tiles, slots[dev & 63]);
     cfg.gridDim = dim3(PAIR ? 2 * units : units, 1, 1);
     cfg.stream = s;
-    ANCHA_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, p));
+    ANCHA_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tsa, tsb, to, tr, p));
     return check_launch("mx_linear");
+}
+
+template <int FMT, int BN, bool PAIR>
+int launch(const MxLinear& q, const Params& p, cudaStream_t s) {
+    return p.res_mode == RES_TMA ? launch<FMT, BN, PAIR, true>(q, p, s) : launch<FMT, BN, PAIR, false>(q, p, s);
 }
 
 template <int FMT>
 int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
     const int64_t row_tiles = p.m <= 64 ? 1 : ceil_div(p.m, 128), tiles = row_tiles * ceil_div(p.n, 128);
-    if (p.m <= 64 || tiles <= 300) {
+    if (p.m <= 64 || tiles <= 74) {
         const int slabs = (int)ceil_div(p.kbytes, SLAB);
         int splits = 1;
         while (splits < 8 && 2 * splits <= slabs && tiles * 2 * splits <= 296) splits *= 2;
@@ -883,8 +969,11 @@ int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
         return launch_split<FMT, 128>(q, p, splits, s);
     }
     if (p.m > 128 && p.n > 128) {
-        // The tile width that pads n less.
-        if (ceil_div(p.n, 192) * 192 < ceil_div(p.n, 256) * 256) return launch<FMT, 192, true>(q, p, s);
+        // 192 columns a tile, with two whole accumulators in TMEM, where the epilogue is the limit (up to 16 slabs of K) or
+        // where they pad n less; else 256, whose operands make fewer bytes (measured, 192 / 256: 48060x1536x384 mxf8
+        // gelu 70 / 83 us, 16384x2048x2048 mxf8 80 / 98 us, 8192^3 mxf8 480 / 447 us and nvf4 267 / 236 us).
+        if (ceil_div(p.kbytes, SLAB) <= 16 || ceil_div(p.n, 192) * 192 < ceil_div(p.n, 256) * 256)
+            return launch<FMT, 192, true>(q, p, s);
         return launch<FMT, 256, true>(q, p, s);
     }
     return launch<FMT, 128, false>(q, p, s);
@@ -901,13 +990,16 @@ int mx_linear(const MxLinear& q, cudaStream_t s) {
     p.gx = q.x.global_scale; p.gw = q.w.global_scale;
     p.bias = q.bias;
     p.residual = q.residual; p.ldr = q.ldr; p.res_type = q.res_type;
-    p.res_vec = q.residual && aligned16(q.residual) && q.ldr * (int64_t)elt_size(q.res_type) % 16 == 0;
+    p.res_mode = !q.residual ? RES_NONE
+                 : aligned16(q.residual) && q.ldr * (int64_t)elt_size(q.res_type) % 16 == 0 ? RES_TMA : RES_ELEMENT;
+    p.rows_padded = (int)(ceil_div(p.m, 128) * 128);
     p.act = q.act;
     p.out = q.out; p.ldo = q.ldo; p.out_type = q.out_type;
     if (q.out_mx) {
         p.out_mode = OUT_MX;
         p.om = *q.out_mx;
         p.okt = (int)mx_ktiles(p.om.format, p.om.cols);
+        p.oblock_log2 = p.om.format == NVF4 ? 4 : 5;
     } else {
         p.out_mode = aligned16(q.out) && q.ldo * (int64_t)elt_size(q.out_type) % 16 == 0 ? OUT_TMA : OUT_PLAIN;
     }
