@@ -39,7 +39,7 @@ struct Shape {
     static constexpr int STAGE = OPERAND_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
     static constexpr int EPI = BN / 16;                 // epilogue warps: 32 rows by 64 columns of the tile each
     static constexpr int THREADS = 64 + 32 * EPI;
-    // Stages and bytes of shared memory; with a residual that TMA can read each epilogue warp has a second buffer.
+    // Stages and bytes of shared memory; with a residual each epilogue warp has a second buffer.
     static constexpr int FIXED = 1024 + 512 + EPI * (STAGING + BIAS_BYTES);
     static constexpr int stages(bool residual) {
         const int fit = (227 * 1024 - FIXED - (residual ? EPI * STAGING : 0)) / STAGE;
@@ -173,11 +173,7 @@ __device__ __forceinline__ void gelu2(float& x0, float& x1) {
     x1 = fmaf(-fabsf(x1), ex2_approx(r1), fmaxf(x1, 0.f));
 }
 
-__device__ __forceinline__ float residual_at(const Params& p, int64_t i) {
-    return p.res_type == ELT_F32    ? static_cast<const float*>(p.residual)[i]
-           : p.res_type == ELT_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[i])
-                                    : __half2float(static_cast<const __half*>(p.residual)[i]);
-}
+__device__ void add_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane, float (&v)[32]);
 
 // v[j ..] += four f32, or eight elements of 16 bits.
 __device__ __forceinline__ void add4(const float4& q, float (&v)[32], int j) {
@@ -196,12 +192,12 @@ __device__ __forceinline__ void add8(const uint4& q, int type, float (&v)[32], i
 }
 
 // act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them); `bias`: theirs, in shared
-// memory, as with RES `res`, the rows of the residual (32 columns of f32, or 64 of 16 bits of which half `half`). The
+// memory, as with RES the buffer `res`: the rows of the residual (32 columns of f32, or 64 of 16 bits of which half `half`), or with RES_ELEMENT its exchange. The
 // arithmetic
 // runs on packed pairs, one instruction for two values: the epilogue is bound by instruction issue.
 template <bool SCALED, bool RES>
-__device__ __forceinline__ void finish32(const Params& p, const float* bias, const uint8_t* res, int half, int lane, int64_t row,
-                                         bool live, int c0, int nv, float alpha, const uint32_t (&r)[32], float (&v)[32]) {
+__device__ __forceinline__ void finish32(const Params& p, const float* bias, uint8_t* res, int half, int lane,
+                                         int64_t row0, int c0, int nv, float alpha, const uint32_t (&r)[32], float (&v)[32]) {
     const uint64_t al = f2(alpha, alpha);
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
@@ -218,7 +214,9 @@ __device__ __forceinline__ void finish32(const Params& p, const float* bias, con
 #pragma unroll
         for (int j = 0; j < 32; j += 2) tanh_fast2(v[j], v[j + 1]);
     }
-    if (RES) {
+    if (RES && p.res_mode == RES_ELEMENT) {
+        add_plain(p, reinterpret_cast<float*>(res), row0, c0, nv, lane, v);
+    } else if (RES) {
         if (p.res_type == ELT_F32) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
@@ -228,10 +226,6 @@ __device__ __forceinline__ void finish32(const Params& p, const float* bias, con
             for (int q = 0; q < 4; ++q)
                 add8(*reinterpret_cast<const uint4*>(res + lane * 128 + (((q + 4 * half) ^ (lane & 7)) * 16)), p.res_type, v, 8 * q);
         }
-    } else if (p.res_mode != RES_NONE && live) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < nv) v[j] += residual_at(p, row * p.ldr + c0 + j);
     }
     if (nv < 32) {
 #pragma unroll
@@ -307,17 +301,56 @@ __device__ __forceinline__ void stage_row(uint8_t* buf, int lane, int type, int 
     }
 }
 
-// Outputs that a TMA store cannot reach (odd addresses or strides): transposed through shared memory so that
-// a warp writes 32 neighbouring columns of a row at a time.
+// Outputs and residuals at odd addresses or strides, an element at a time: exchanged through the buffer (a lane's row
+// there, columns rotated by the row against bank conflicts) so that a warp touches 32 neighbouring columns of a row,
+// eight rows in flight.
+template <typename T>
+__device__ __forceinline__ void store_rows(T* out, int64_t ld, int rows, int nv, int lane, const float* buf) {
+    if (lane >= nv) return;
+#pragma unroll 1
+    for (int r = 0; r < rows; r += 8) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = buf[(r + k) * 32 + (lane ^ (r + k))];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (r + k < rows) store_f(out + (r + k) * ld + lane, x[k]);
+    }
+}
 __device__ __forceinline__ void store_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane,
                                             const float (&v)[32]) {
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 32; ++j) buf[lane * 32 + (j ^ lane)] = v[j];
     __syncwarp();
-    if (lane >= nv) return;
-    for (int r = 0; r < 32 && row0 + r < p.m; ++r)
-        store_elt(p.out, (row0 + r) * p.ldo + c0 + lane, buf[r * 32 + (lane ^ r)], p.out_type);
+    const int rows = (int)min((int64_t)32, p.m - row0);
+    const int64_t at = row0 * p.ldo + c0;
+    if (p.out_type == ELT_F32) store_rows(static_cast<float*>(p.out) + at, p.ldo, rows, nv, lane, buf);
+    else if (p.out_type == ELT_BF16) store_rows(static_cast<__nv_bfloat16*>(p.out) + at, p.ldo, rows, nv, lane, buf);
+    else store_rows(static_cast<__half*>(p.out) + at, p.ldo, rows, nv, lane, buf);
+}
+template <typename T>
+__device__ __forceinline__ void load_rows(const T* in, int64_t ld, int rows, int nv, int lane, float* buf) {
+#pragma unroll 1
+    for (int r = 0; r < 32; r += 8) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = r + k < rows && lane < nv ? load_f(in + (r + k) * ld + lane) : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) buf[(r + k) * 32 + (lane ^ (r + k))] = x[k];
+    }
+}
+__device__ __forceinline__ void add_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane, float (&v)[32]) {
+    const int rows = (int)min((int64_t)32, p.m - row0);
+    const int64_t at = row0 * p.ldr + c0;
+    __syncwarp();
+    if (p.res_type == ELT_F32) load_rows(static_cast<const float*>(p.residual) + at, p.ldr, rows, nv, lane, buf);
+    else if (p.res_type == ELT_BF16) load_rows(static_cast<const __nv_bfloat16*>(p.residual) + at, p.ldr, rows, nv, lane, buf);
+    else load_rows(static_cast<const __half*>(p.residual) + at, p.ldr, rows, nv, lane, buf);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += buf[lane * 32 + (j ^ lane)];
+    __syncwarp();
 }
 
 // A lane's 32 columns quantised, one block of 32 or two of 16, in its registers; the codes go to its row of the staging
@@ -537,7 +570,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
         };
         if (p.bias && tile0 < p.tiles) load_bias(walk.ni);
         // The residual's 32 x 32 f32, or 32 x 64 elements of 16 bits, in the layout of the staging buffer.
-        const bool res_wide = p.res_type == ELT_F32;
+        const bool res_tma = p.res_mode == RES_TMA, res_wide = p.res_type == ELT_F32;
         uint32_t res_phase = 0;
         bool res_pending = false;
         const auto load_res = [&](int c, int64_t row0) {
@@ -559,7 +592,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             bias[lane] = b0;
             bias[32 + lane] = b1;
             if (p.bias && t + tstep < p.tiles) load_bias(walk.ni);
-            if (RES && some) load_res(c_first, row0);
+            if (RES && res_tma && some) load_res(c_first, row0);
             if (!warp_wait(&tfull[b], (local >> 1) & 1, abort, p.err)) break;
             tc_fence_after();
             const uint32_t base = tmem + b * S::ACC1 + col0 + ((uint32_t)(quarter * 32) << 16);
@@ -581,19 +614,19 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 const int c0 = c_first + 32 * h, nv = min(32, p.n - c0);
                 if (nv <= 0 || !some) continue;
                 float v[32];
+                if (p.out_mode != OUT_PLAIN && (wide || h == 0)) {
+                    if (elect_one()) bulk_wait_read<0>();  // the store that last read the buffer is done with it
+                    __syncwarp();
+                }
                 if (RES && res_pending) {
                     res_ok = warp_wait(rbar, res_phase, abort, p.err);
                     if (!res_ok) break;
                     res_phase ^= 1;
                     res_pending = false;
                 }
-                finish32<FMT == NVF4, RES>(p, bias + 32 * h, res, h, lane, row, row < p.m, c0, nv, alpha, r[h], v);
-                if (RES && res_wide && h == 0 && c0 + 32 < p.n) load_res(c0 + 32, row0);
+                finish32<FMT == NVF4, RES>(p, bias + 32 * h, res, h, lane, row0, c0, nv, alpha, r[h], v);
+                if (RES && res_tma && res_wide && h == 0 && c0 + 32 < p.n) load_res(c0 + 32, row0);
                 if (p.out_mode == OUT_TMA) {
-                    if (wide || h == 0) {  // the store that last read the buffer is done with it
-                        if (elect_one()) bulk_wait_read<0>();
-                        __syncwarp();
-                    }
                     stage_row(stage, lane, p.out_type, h, v);
                     if (wide) {
                         fence_proxy_async();
@@ -606,10 +639,6 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 } else if (p.out_mode == OUT_PLAIN) {
                     store_plain(p, reinterpret_cast<float*>(stage), row0, c0, nv, lane, v);
                 } else {
-                    if (h == 0) {
-                        if (elect_one()) bulk_wait_read<0>();
-                        __syncwarp();
-                    }
                     if (p.om.format == MXF8) codes |= stage_mx<MXF8>(p.om, stage, h, lane, v) << (8 * h);
                     else if (p.om.format == MXF4) codes |= stage_mx<MXF4>(p.om, stage, h, lane, v) << (8 * h);
                     else codes |= stage_mx<NVF4>(p.om, stage, h, lane, v) << (16 * h);
@@ -630,8 +659,13 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 if (row < p.rows_padded && blk / 4 < p.okt) {
                     uint8_t* sc = p.om.scales + mx_scale_word(row, blk / 4, p.okt) + blk % 4;
                     if (row >= p.m) codes = 0;
-                    if (p.oblock_log2 == 5) *reinterpret_cast<uint16_t*>(sc) = (uint16_t)codes;
-                    else *reinterpret_cast<uint32_t*>(sc) = codes;
+                    if (p.oblock_log2 == 5) {
+                        *reinterpret_cast<uint16_t*>(sc) = (uint16_t)codes;
+                        // The last tile may end in the middle of a scale tile's 128 columns: its last warps write the rest.
+                        if (c_first + 64 == p.n_tiles * BN && blk % 4 == 0) *reinterpret_cast<uint16_t*>(sc + 2) = 0;
+                    } else {
+                        *reinterpret_cast<uint32_t*>(sc) = codes;
+                    }
                 }
             }
         }
@@ -893,7 +927,7 @@ int launch_split(const MxLinear& q, const Params& p, int splits, cudaStream_t s)
     return check_launch("mx_linear (split)");
 }
 
-// RES: a residual that TMA can read (the kernel without it keeps its registers).
+// RES: with a residual (the kernel without one keeps its registers and shared memory).
 template <int FMT, int BN, bool PAIR, bool RES>
 int launch(const MxLinear& q, Params p, cudaStream_t s) {
     using S = Shape<FMT, BN, PAIR>;
@@ -937,7 +971,7 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
     else if (p.out_mode == OUT_TMA)
         ANCHA_TRY(make_tma_store_3d(&to, p.out, p.out_type, p.n, p.m, 1, p.ldo, (int64_t)p.m * p.ldo, p.out_type == ELT_F32 ? 32 : 64, 32));
     CUtensorMap tr = ta;
-    if (RES)
+    if (p.res_mode == RES_TMA)
         ANCHA_TRY(make_tma_store_3d(&tr, p.residual, p.res_type, p.n, p.m, 1, p.ldr, (int64_t)p.m * p.ldr,
                                     p.res_type == ELT_F32 ? 32 : 64, 32));
     p.m_tiles = (int)ceil_div(p.m, PAIR ? 2 * BM : BM);
@@ -954,14 +988,17 @@ int launch(const MxLinear& q, Params p, cudaStream_t s) {
 
 template <int FMT, int BN, bool PAIR>
 int launch(const MxLinear& q, const Params& p, cudaStream_t s) {
-    return p.res_mode == RES_TMA ? launch<FMT, BN, PAIR, true>(q, p, s) : launch<FMT, BN, PAIR, false>(q, p, s);
+    return p.res_mode != RES_NONE ? launch<FMT, BN, PAIR, true>(q, p, s) : launch<FMT, BN, PAIR, false>(q, p, s);
 }
 
 template <int FMT>
 int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
+    // Split where the rows fill no tile, or the tiles are few and K is long (measured, split / whole tiles: 2000x64x8192
+    // nvf4 12 / 17 us, 133x1544x1000 mxf8 9.4 / 10.5 us; 65x1536x384 7.2 / 5.4 us, 128x4096x4096 mxf4 12.3 / 10.6 us). Of
+    // 1, 2, 4 or 8 parts the most that leave each a slab and need no more than two CTAs per SM.
+    const int slabs = (int)ceil_div(p.kbytes, SLAB);
     const int64_t row_tiles = p.m <= 64 ? 1 : ceil_div(p.m, 128), tiles = row_tiles * ceil_div(p.n, 128);
-    if (p.m <= 64 || tiles <= 74) {
-        const int slabs = (int)ceil_div(p.kbytes, SLAB);
+    if (p.m <= 64 || (tiles <= 30 && slabs >= 8)) {
         int splits = 1;
         while (splits < 8 && 2 * splits <= slabs && tiles * 2 * splits <= 296) splits *= 2;
         if (p.m <= 16) return launch_split<FMT, 16>(q, p, splits, s);
@@ -972,7 +1009,7 @@ int by_shape(const MxLinear& q, const Params& p, cudaStream_t s) {
         // 192 columns a tile, with two whole accumulators in TMEM, where the epilogue is the limit (up to 16 slabs of K) or
         // where they pad n less; else 256, whose operands make fewer bytes (measured, 192 / 256: 48060x1536x384 mxf8
         // gelu 70 / 83 us, 16384x2048x2048 mxf8 80 / 98 us, 8192^3 mxf8 480 / 447 us and nvf4 267 / 236 us).
-        if (ceil_div(p.kbytes, SLAB) <= 16 || ceil_div(p.n, 192) * 192 < ceil_div(p.n, 256) * 256)
+        if (slabs <= 16 || ceil_div(p.n, 192) * 192 < ceil_div(p.n, 256) * 256)
             return launch<FMT, 192, true>(q, p, s);
         return launch<FMT, 256, true>(q, p, s);
     }

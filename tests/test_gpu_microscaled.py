@@ -26,6 +26,19 @@ DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
+@pytest.fixture(autouse=True)
+def poisoned_memory(monkeypatch):
+    """New arrays hold 0xAB everywhere, so that a byte that a call has to write and does not is seen."""
+    plain = mx.Microscaled._new.__func__
+
+    def poisoned(cls, *args):
+        q = plain(cls, *args)
+        q._buffer.fill_(0xAB)
+        return q
+
+    monkeypatch.setattr(mx.Microscaled, "_new", classmethod(poisoned))
+
+
 def f64(t):
     return t.detach().double().cpu().numpy()
 
@@ -405,7 +418,8 @@ def test_linear_strides_and_offsets(fmt, m, n):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("out", FORMATS)
-@pytest.mark.parametrize("m,n,k", [(1, 1, 40), (1, 512, 256), (30, 100, 96), (129, 300, 384), (256, 515, 200), (384, 768, 128)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 40), (1, 512, 256), (30, 100, 96), (129, 300, 384), (256, 515, 200), (384, 768, 128),
+                                   (200, 65, 64), (300, 130, 64), (300, 321, 96), (130, 577, 64), (260, 449, 2080)])
 def test_linear_with_quantized_output(fmt, out, m, n, k):
     """The quantised output is the quantisation of the f32 output, bit for bit."""
     x, w = operands(fmt, m, n, k, 9)
