@@ -151,11 +151,11 @@ __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32
 
 // ---- epilogue -------------------------------------------------------------------------------
 
-// GELU(x) = max(x, 0) - |x| Phi(-|x|) with Phi(-u) = 2^R(u), u = min(|x|, 5.5), R a polynomial in
-// v = u 2/5.5 - 1 of degree 7, fitted here to log2 Phi(-u) with the weight u Phi(-u) that its error has in the result
-// (Lawson's iteration). Evaluated in f32 the error is f32's own: rms 5.3e-8 on [-4, 4], 2.5e-7 at most (the
+// GELU(x) = max(x, 0) - u Phi(-u) with u = min(|x|, 5.5) (beyond, u Phi(-u) < 1.1e-7), Phi(-u) = 2^R(u), R a polynomial
+// in v = u 2/5.5 - 1 of degree 7, fitted here to log2 Phi(-u) with the weight u Phi(-u) that its error has in the result
+// (Lawson's iteration). Evaluated in f32 the error is f32's own: rms 5.3e-8 on [-4, 4], 2.5e-7 at most up to |x| = 12 (the
 // 16-bit epilogues' fit of the same degree, weighted for log2 Phi itself, has 7e-7, which moves the codes of a
-// quantised output more often than the product's own rounding). The coefficients lie in constant memory as pairs: as
+// quantised output more often than the product's own rounding). NaN stays NaN. The coefficients lie in constant memory as pairs: as
 // immediates each would cost the packed FMA two moves.
 __constant__ float2 kGelu[8] = {{-8.390578269958496f, -8.390578269958496f}, {-12.107535362243652f, -12.107535362243652f},
                                 {-5.02378511428833f, -5.02378511428833f}, {-0.18455249071121216f, -0.18455249071121216f},
@@ -163,14 +163,17 @@ __constant__ float2 kGelu[8] = {{-8.390578269958496f, -8.390578269958496f}, {-12
                                 {0.015407359227538109f, 0.015407359227538109f}, {0.00019493377476464957f, 0.00019493377476464957f}};
 __device__ __forceinline__ void gelu2(float& x0, float& x1) {
     const uint64_t* c = reinterpret_cast<const uint64_t*>(kGelu);
-    const uint64_t v = ffma2(f2(fminf(fabsf(x0), 5.5f), fminf(fabsf(x1), 5.5f)), f2(2.0f / 5.5f, 2.0f / 5.5f), f2(-1.0f, -1.0f));
+    float u0, u1;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(u0) : "f"(fabsf(x0)), "f"(5.5f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(u1) : "f"(fabsf(x1)), "f"(5.5f));
+    const uint64_t v = ffma2(f2(u0, u1), f2(2.0f / 5.5f, 2.0f / 5.5f), f2(-1.0f, -1.0f));
     uint64_t r = c[7];
 #pragma unroll
     for (int i = 6; i >= 0; --i) r = ffma2(r, v, c[i]);
     float r0, r1;
     f2_split(r, r0, r1);
-    x0 = fmaf(-fabsf(x0), ex2_approx(r0), fmaxf(x0, 0.f));
-    x1 = fmaf(-fabsf(x1), ex2_approx(r1), fmaxf(x1, 0.f));
+    x0 = fmaf(-u0, ex2_approx(r0), fmaxf(x0, 0.f));
+    x1 = fmaf(-u1, ex2_approx(r1), fmaxf(x1, 0.f));
 }
 
 __device__ void add_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane, float (&v)[32]);
@@ -191,10 +194,10 @@ __device__ __forceinline__ void add8(const uint4& q, int type, float (&v)[32], i
     }
 }
 
-// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them); `bias`: theirs, in shared
-// memory, as with RES the buffer `res`: the rows of the residual (32 columns of f32, or 64 of 16 bits of which half `half`), or with RES_ELEMENT its exchange. The
-// arithmetic
-// runs on packed pairs, one instruction for two values: the epilogue is bound by instruction issue.
+// act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them). `bias`: theirs, in shared
+// memory; with RES, `res` is the warp's residual buffer: its rows there (32 columns of f32, or 64 of 16 bits of which half
+// `half`), or with RES_ELEMENT room to exchange them. The arithmetic runs on packed pairs, one instruction for two
+// values: the epilogue is bound by instruction issue.
 template <bool SCALED, bool RES>
 __device__ __forceinline__ void finish32(const Params& p, const float* bias, uint8_t* res, int half, int lane,
                                          int64_t row0, int c0, int nv, float alpha, const uint32_t (&r)[32], float (&v)[32]) {

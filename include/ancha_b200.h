@@ -180,7 +180,7 @@ enum { ANCHA_MXF8 = 0, ANCHA_MXF4 = 1, ANCHA_NVF4 = 2 };
  * Calls that write an array write the element bytes of a row up to the next multiple of 16 and every
  * byte of the scale tiles, with zeros behind the last column, row and block; data behind that, and rows
  * behind `rows`, are left as they were. Calls that read one need the scales behind a row's last block to
- * be numbers (not NaN: zeros). `global_scale`: the array scale, one device f32 > 0, or NULL for 1;
+ * be numbers (not NaN: zeros) and, with an odd number of 4-bit columns, the other half of the last byte 0. `global_scale`: the array scale, one device f32 > 0, or NULL for 1;
  * ANCHA_NVF4 only. */
 typedef struct {
     int format;
@@ -236,7 +236,8 @@ typedef struct {
  * format (ancha_linear_fwd's ANCHA_W_NK layout and order of the epilogue), on the block-scaled tensor
  * cores with f32 accumulation. y is written to out (out_dtype), or quantised into out_mx (any format):
  * exactly one of the two. bias: device f32 [n] or NULL; residual may be NULL, or out itself with the same
- * type and row stride. No allocation, no workspace. */
+ * type and row stride; any other overlap of an output with an input is undefined. ANCHA_ACT_GELU is the erf form.
+ * No allocation, no workspace. */
 ANCHA_API int ancha_mx_linear_fwd(const ancha_mx_linear_desc* desc, const ancha_mx_array* x, const ancha_mx_array* w,
                                   const float* bias, const void* residual, void* out, const ancha_mx_array* out_mx,
                                   void* stream);

@@ -456,6 +456,30 @@ def test_linear_with_poisoned_and_empty_rows(fmt, m, n):
     check_linear(mx.quantize(xv[keep], fmt), mx.quantize(wv[keep_n], fmt), bias[keep_n].contiguous())
 
 
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("act", ["gelu", "tanh"])
+def test_activations_at_their_ends(m, act):
+    """Large sums, sums near zero, infinities (an overflowing sum) and NaN through the activations."""
+    k, n = 64, 160
+    w = mx.quantize(torch.eye(n, k, device="cuda"), "mxf8")
+    x = torch.zeros((m, k), device="cuda")
+    tops = [0.0, 1e-30, -1e-30, 1e-4, -1e-4, 3.0, -3.0, 5.5, -5.5, 8.0, -8.0, 256.0, -256.0, 2.0 ** 60, -2.0 ** 60]
+    vals = torch.tensor([tops[i % len(tops)] for i in range(2 * m)], device="cuda").view(m, 2)
+    x[:, 0], x[:, 32] = vals[:, 0], vals[:, 1]  # one value to a block
+    x[1, 1] = math.nan
+    bias = torch.zeros(n, device="cuda")
+    bias[40], bias[41], bias[42] = math.inf, -math.inf, math.nan
+    y = f64(mx.linear(mx.quantize(x, "mxf8"), w, bias, act, dtype=torch.float32))
+    z = f64(mx.dequantize(mx.quantize(x, "mxf8"))) @ f64(mx.dequantize(w)).T + f64(bias)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want = gelu64(z) if act == "gelu" else np.tanh(z)
+    want = np.where(np.isneginf(z), 0.0 if act == "gelu" else -1.0, want)
+    assert np.array_equal(np.isnan(y), np.isnan(want))
+    ok = np.isfinite(want)
+    assert np.array_equal(y[~ok & ~np.isnan(want)], want[~ok & ~np.isnan(want)])
+    assert (np.abs(y[ok] - want[ok]) <= 7e-7 + 5e-6 * np.abs(want[ok])).all()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_linear_is_deterministic_and_rows_are_independent(fmt):
     x, w = operands(fmt, 300, 520, 2000, 12)
