@@ -95,10 +95,9 @@ __device__ __forceinline__ float mx_scale_value(uint32_t code) {
     return FMT == NVF4 ? e4m3_value(code) : e8m0_value(code);
 }
 
-// How a block is quantised: the code of its scale, and each element as v * mul (a power of two, exact)
-// or v / div (NVF4, whose divisor is no power of two: a division rounds next to a border of the grid as
-// the quotient does, a multiplication by the reciprocal does not). A block with an infinity or a NaN
-// has the scale NaN and elements 0; `live` is false for it, and where the divisor is 0.
+// How a block is quantised: the code of its scale, and each element as v * factor (MX: a power of two, exact) or
+// v / factor (NVF4). A block with an infinity or a NaN has the scale NaN and elements 0; `live` is false for it, and
+// where the divisor is 0.
 struct MxBlock {
     uint32_t code;
     float factor;

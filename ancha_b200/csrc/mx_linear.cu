@@ -7,10 +7,14 @@
 // copy wants. One K slab is 128 bytes of a row in every format (128 elements of 8 bits, 256 of 4), four
 // instructions; it needs 1 (mxf8), 2 (mxf4) or 4 (nvf4) scale tiles per 128 rows.
 //
-// Persistent and warp-specialised, as the 16-bit GEMM: warp 0 loads slabs of both operands and their
-// scales by TMA through a ring of stages, warp 1 issues the copies and products, the other warps drain
-// the accumulator. A CTA pair shares a 256 x 256 tile (each CTA holds 128 rows of x, half of w's rows, and
-// all of w's scales).
+// Persistent and warp-specialised, as the 16-bit GEMM: warp 0 loads slabs of both operands and their scales by TMA
+// through a ring of stages, warp 1 issues the copies and products, the other warps drain the accumulator (32 rows by 64
+// columns each). A CTA pair shares a tile of 256 rows by 192 or 256 columns (each CTA holds 128 rows of x, half of w's rows,
+// and all of w's scales). Few rows, or few tiles with long K, take the split kernel at the end.
+//
+// Measured (one B200): 8192^3 nvf4 233 us = 4.7 PFLOP/s, mxf4 200 us = 5.5, mxf8 437 us = 2.5 under the power cap, where the
+// tensor pipe and the scale copies are the limit (a slab's 512 cycles of products and 3, 6 or 12 copies); 48060 x 1536 x 384
+// mxf8 with GELU into mxf8 72 us, where the epilogue's arithmetic is (44 us without GELU); 1 x 4096 x 4096 mxf4 7 us, latency.
 #include "mx.cuh"
 #include "tc.cuh"
 
