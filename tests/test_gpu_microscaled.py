@@ -22,6 +22,7 @@ from ancha_b200 import microscaled as mx  # noqa: E402
 from oracle import microscaled as O  # noqa: E402
 
 FORMATS = ("mxf8", "mxf4", "nvf4")
+BLOCK = O.BLOCK
 DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
@@ -237,6 +238,20 @@ def test_offsets_beyond_32_bits():
     assert (y[:-300] == 1).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_very_wide_rows(fmt):
+    """Two rows of fifty million columns: their blocks are those of the same elements in short rows."""
+    cols, whole = 50_000_001, 49_999_872
+    x = rows_of(2, 4096, torch.bfloat16, seed=3).repeat(1, cols // 4096 + 1)[:, :cols]
+    q, short = mx.quantize(x, fmt), mx.quantize(x[:, :whole].reshape(-1, 1024), fmt)
+    n = whole if fmt == "mxf8" else whole // 2
+    assert torch.equal(q.data[:, :n].reshape(-1), short.data.reshape(-1))
+    assert torch.equal(q.scale_codes()[:, :whole // BLOCK[fmt]].reshape(-1), short.scale_codes().reshape(-1))
+    assert torch.equal(mx.dequantize(q, torch.bfloat16)[:, :whole].reshape(-1, 1024), mx.dequantize(short, torch.bfloat16))
+    tail = mx.quantize(x[:, whole:].contiguous(), fmt)
+    assert torch.equal(mx.dequantize(q)[:, whole:], mx.dequantize(tail))
+
+
 # ---------------------------------------------------------------------------------------- norm
 
 def check_norm(x, residual, gain, eps, fmt, g=None, **kw):
@@ -285,6 +300,19 @@ def test_add_rms_norm_in_place_and_strided():
         assert torch.equal(q.data, want.data) and torch.equal(q.scales, want.scales)
         whole[:, lo:lo + dim] = s
         assert torch.equal(r._base, whole)
+
+
+@pytest.mark.parametrize("dim", [600, 1501, 5003, 20001])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_add_rms_norm_in_place_at_odd_widths(dim, kind):
+    """The stream written over the residual, and over x, where rows cannot be read in vectors."""
+    x, r = rows_of(5, dim, DTYPES[kind], 1), rows_of(5, dim, DTYPES[kind], 2)
+    want, s = mx.add_rms_norm(x, r)
+    for over in (0, 1):
+        a, b = x.clone(), r.clone()
+        q, s2 = mx.add_rms_norm(a, b, residual_out=(b, a)[over])
+        assert torch.equal(s2, s) and torch.equal(q.data, want.data) and torch.equal(q.scales, want.scales)
+        assert torch.equal((a, b)[over], (x, r)[over])  # the other one as it was
 
 
 def test_add_rms_norm_does_not_depend_on_the_split():
@@ -486,6 +514,36 @@ def test_linear_is_deterministic_and_rows_are_independent(fmt):
     y = mx.linear(x, w, dtype=torch.float32)
     for _ in range(5):
         assert torch.equal(mx.linear(x, w, dtype=torch.float32), y)
+
+
+@pytest.mark.parametrize("n", [32768, 32771])
+@pytest.mark.parametrize("kind", ["bf16", "mxf8", "mxf4"])
+def test_linear_outputs_beyond_32_bits(n, kind):
+    """An output of more than 2^31 elements: its last rows against float64."""
+    m, k = 70016, 32
+    x, w = operands("mxf8", m, n, k, 4)
+    bias = rows_of(1, n, torch.float32, 5)[0]
+    last = mx.quantize(mx.dequantize(x)[-100:], "mxf8")  # values of the format: quantised to themselves
+    assert torch.equal(mx.dequantize(last), mx.dequantize(x)[-100:])
+    y, tol = linear64(last, w, bias)
+    if kind == "bf16":
+        got = f64(mx.linear(x, w, bias)[-100:])
+        assert (np.abs(got - y) <= tol + 2.0 ** -8 * (np.abs(y) + tol)).all()
+        return
+    q = mx.linear(x, w, bias, format=kind)
+    width = -(-(n if kind == "mxf8" else (n + 1) // 2) // 16) * 16
+    tail = mx.empty(kind, 100, n)
+    tail.data.copy_(q.data[-100:, :width])
+    codes = q.scale_codes()[-100:].cpu().numpy()
+    tail.scales.copy_(torch.from_numpy(O.tile(codes)).view(tail.scales.shape))
+    check_near(tail, y, tol)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [2, 200])
+def test_linear_with_a_very_long_depth(fmt, m):
+    x, w = operands(fmt, m, 5, 300_001, 6)
+    check_linear(x, w)
 
 
 # ------------------------------------------------------------------------------------- together
