@@ -142,23 +142,29 @@ def _matrix(t, device: int, name: str):
 
 
 def _array(q: Microscaled, device: int, name: str) -> N.MxArray:
-    ld, shape, data_bytes, _ = _layout(q.format, q.rows, q.cols)
-    g = None if q.global_scale is None else _vector(q.global_scale, device, 1, f"{name}: global_scale")
+    fmt, rows, cols = q.format, q.rows, q.cols
+    ld, shape, data_bytes, _ = _layout(fmt, rows, cols)
+    g = q.global_scale
+    if g is not None:
+        g = _vector(g, device, 1, f"{name}: global_scale")
     buffer = q._buffer
     if buffer is not None:
-        _on(buffer, device, name)
+        if buffer.get_device() != device:
+            raise _invalid(f"{name}: not on the device of the first operand")
         at = buffer.data_ptr()
-        return N.MxArray(FORMATS[q.format], q.rows, q.cols, at, ld, at + data_bytes, g)
+        return N.MxArray(FORMATS[fmt], rows, cols, at, ld, at + data_bytes, g)
     data, scales = q._data, q._scales
-    if data.dtype != torch.uint8 or data.dim() != 2 or data.shape[0] != q.rows or data.shape[1] < ld \
-            or data.stride(1) != 1:
-        raise _invalid(f"{name}: data is not uint8 [{q.rows}, >= {ld}] with contiguous rows")
-    if scales.dtype != torch.uint8 or scales.shape != shape or not scales.is_contiguous():
+    if data.dtype is not torch.uint8 or data.shape != (rows, ld) or not data.is_contiguous():
+        if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[0] != rows or data.shape[1] < ld \
+                or data.stride(1) != 1:
+            raise _invalid(f"{name}: data is not uint8 [{rows}, >= {ld}] with contiguous rows")
+        if rows > 1:
+            ld = data.stride(0)
+    if scales.dtype is not torch.uint8 or scales.shape != shape or not scales.is_contiguous():
         raise _invalid(f"{name}: scales are not contiguous uint8 {shape}")
-    _on(data, device, name)
-    _on(scales, device, name)
-    return N.MxArray(FORMATS[q.format], q.rows, q.cols, data.data_ptr(), data.stride(0) if q.rows > 1 else ld,
-                     scales.data_ptr(), g)
+    if data.get_device() != device or scales.get_device() != device:
+        raise _invalid(f"{name}: not on the device of the first operand")
+    return N.MxArray(FORMATS[fmt], rows, cols, data.data_ptr(), ld, scales.data_ptr(), g)
 
 
 def _run(device: int, fn, *args):
