@@ -8,6 +8,7 @@
 #include "mx.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace ancha {
 namespace {
@@ -307,8 +308,16 @@ __device__ __forceinline__ void add_squares(uint64_t& sum, uint64_t& err, uint64
 }
 
 // 1 / sqrt(x) in f64, rounded to f32: the f32 estimate (2 ulp) and one Newton step in f64, which squares its error.
-__device__ __forceinline__ float inverse_root(double x) {
-    if (!(x > 1e-30 && x < 1e30)) return (float)(1.0 / sqrt(x));
+// The result leaves f32's normal numbers for rows of subnormal numbers (up to 1e47) or of the largest ones (down to
+// 3e-39), and for rows of zeros, where it is 1 / sqrt(eps), whatever that is. Towards these ends a power of two of it,
+// `pre`, is left to the row's elements, which take it exactly, and what is still too large (zeros) is f32's largest number.
+__device__ __forceinline__ float inverse_root(double x, float& pre) {
+    pre = 1.f;
+    if (!(x > 1e-30 && x < 1e30)) {
+        pre = x < 1.0 ? 0x1p64f : 0x1p-24f;
+        const double r = 1.0 / (sqrt(x) * pre);
+        return r > FLT_MAX ? FLT_MAX : (float)r;  // NaN stays
+    }
     const double r = rsqrtf((float)x);
     return (float)fma(0.5 * r, fma(-x * r, r, 1.0), r);
 }
@@ -402,7 +411,14 @@ add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
 #pragma unroll
         for (int i = 0; i < W; ++i) d += part[warp / W * W + i];
     }
-    const float inv = inverse_root(d * a.inv_cols + a.eps);
+    float pre;
+    const float inv = inverse_root(d * a.inv_cols + a.eps, pre);
+    if (pre != 1.f) {  // the same for all of a row's threads
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[i][j] *= pre;
+    }
     const float g = FMT == NVF4 && a.o.global_scale ? *a.o.global_scale : 1.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
