@@ -180,6 +180,25 @@ __device__ __forceinline__ void gelu2(float& x0, float& x1) {
     x1 = fmaf(-u1, ex2_approx(r1), fmaxf(x1, 0.f));
 }
 
+// tanh(x) with a relative error below 1e-6 everywhere, since an output with block scales keeps small numbers' relative
+// precision: 1 - 2 / (e^2x + 1) from |x| = 0.5 on (its error of up to 4e-7 is absolute: at 1e-6 it would be a sixth of the
+// result), below it x + x^3 P(x^2), P of degree 3 fitted here to the least relative error (linear programming; 8e-8 in
+// f32's steps). 48060 x 1536 x 384 mxf8 -> bf16: 74 us, 64 us without the polynomial.
+__constant__ float2 kTanh[4] = {{-0.333331435918808f, -0.333331435918808f}, {0.13325878977775574f, 0.13325878977775574f},
+                                {-0.05304549261927605f, -0.05304549261927605f}, {0.01724149100482464f, 0.01724149100482464f}};
+__device__ __forceinline__ void tanh2(float& x0, float& x1) {
+    const uint64_t* c = reinterpret_cast<const uint64_t*>(kTanh);
+    const uint64_t x = f2(x0, x1), z = fmul2(x, x);
+    uint64_t r = c[3];
+#pragma unroll
+    for (int i = 2; i >= 0; --i) r = ffma2(r, z, c[i]);
+    float s0, s1, t0 = x0, t1 = x1;
+    f2_split(ffma2(fmul2(x, z), r, x), s0, s1);
+    tanh_fast2(t0, t1);
+    x0 = fabsf(x0) < 0.5f ? s0 : t0;
+    x1 = fabsf(x1) < 0.5f ? s1 : t1;
+}
+
 __device__ void add_plain(const Params& p, float* buf, int64_t row0, int c0, int nv, int lane, float (&v)[32]);
 
 // v[j ..] += four f32, or eight elements of 16 bits.
@@ -219,7 +238,7 @@ __device__ __forceinline__ void finish32(const Params& p, const float* bias, uin
         for (int j = 0; j < 32; j += 2) gelu2(v[j], v[j + 1]);
     } else if (p.act == ANCHA_ACT_TANH) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) tanh_fast2(v[j], v[j + 1]);
+        for (int j = 0; j < 32; j += 2) tanh2(v[j], v[j + 1]);
     }
     if (RES && p.res_mode == RES_ELEMENT) {
         add_plain(p, reinterpret_cast<float*>(res), row0, c0, nv, lane, v);
@@ -879,8 +898,8 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
             gelu2(v[0], v[1]);
             gelu2(v[2], v[3]);
         } else if (p.act == ANCHA_ACT_TANH) {
-            tanh_fast2(v[0], v[1]);
-            tanh_fast2(v[2], v[3]);
+            tanh2(v[0], v[1]);
+            tanh2(v[2], v[3]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = j < nv ? v[j] + res[j] : 0.f;

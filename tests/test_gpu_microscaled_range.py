@@ -1,4 +1,10 @@
-"""Microscaled operators at the ends of the value range, against float64. Tolerances are test_gpu_microscaled.py's."""
+"""Microscaled operators at the ends of the value range, against float64.
+
+Tolerances, beside test_gpu_microscaled.py's. The inputs of the activations here are sums of one product, which are
+exact, so what is off is the activation alone:
+
+* tanh: relative 1e-6 (below 0.5 an odd polynomial, off by less than 1e-7 in f32; above it 1 - 2 / (e^2x + 1), whose
+  exponential is off by 2^-22, whose reciprocal by 2^-23 and whose other steps by 2^-24 each, so 9.1e-7 of tanh)."""
 import numpy as np
 import pytest
 
@@ -7,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 from ancha_b200 import microscaled as mx  # noqa: E402
 from oracle import microscaled as O  # noqa: E402
-from test_gpu_microscaled import FORMATS, check_near, f64, poisoned_memory, rows_of  # noqa: E402,F401
+from test_gpu_microscaled import FORMATS, check_near, f64, poisoned_memory, rows_of, scalar  # noqa: E402,F401
 
 
 # ---------------------------------------------------------------------------------------- norm
@@ -28,3 +34,41 @@ def test_norm_of_zero_and_extreme_rows_with_any_eps(fmt, dim):
         q, _ = mx.add_rms_norm(x, None, None, eps, fmt)
         assert not f64(mx.dequantize(q))[0].any()
         check_near(q, y, 4 * 2.0 ** -24 * np.abs(y))
+
+
+# --------------------------------------------------------------------------------- activations
+
+def sums(m, top):
+    """x and w whose product is x itself: [m, 256] numbers up to about 4 `top`, a row of one size each, from `top` down
+    by 2^-40 over the rows, their blocks' elements from full size to nothing."""
+    k = 256
+    rng = np.random.default_rng(m)
+    v = rng.standard_normal((m, k)) * np.exp2(-rng.uniform(0, 8, (m, k))) * np.exp2(-40 * np.arange(m) / m)[:, None] * top
+    x = mx.quantize(torch.from_numpy(v).float().cuda(), "mxf8")
+    return x, mx.quantize(torch.eye(k, device="cuda"), "mxf8"), f64(mx.dequantize(x))
+
+
+def activation(act, z):
+    """(activation, tolerance) in float64."""
+    y = np.tanh(z)
+    return y, 1e-6 * np.abs(y)
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+@pytest.mark.parametrize("act", ["tanh"])
+@pytest.mark.parametrize("top", [4.0, 0.05])
+def test_activations_over_their_range(m, act, top):
+    x, w, z = sums(m, top)
+    y, tol = activation(act, z)
+    got = f64(mx.linear(x, w, None, act, dtype=torch.float32))
+    assert (np.abs(got - y) <= tol).all(), float((np.abs(got - y) / (tol + 1e-300)).max())
+
+
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_small_tanh_keeps_its_blocks(m, fmt):
+    """Blocks of small sums, whose scale and codes are those of tanh and not of its rounding."""
+    x, w, z = sums(m, 0.05)
+    y, tol = activation("tanh", z)
+    g = 2.0 ** -30 if fmt == "nvf4" else None
+    check_near(mx.linear(x, w, None, "tanh", format=fmt, global_scale=scalar(g)), y, tol)
