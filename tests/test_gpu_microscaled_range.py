@@ -4,7 +4,12 @@ Tolerances, beside test_gpu_microscaled.py's. The inputs of the activations here
 exact, so what is off is the activation alone:
 
 * tanh: relative 1e-6 (below 0.5 an odd polynomial, off by less than 1e-7 in f32; above it 1 - 2 / (e^2x + 1), whose
-  exponential is off by 2^-22, whose reciprocal by 2^-23 and whose other steps by 2^-24 each, so 9.1e-7 of tanh)."""
+  exponential is off by 2^-22, whose reciprocal by 2^-23 and whose other steps by 2^-24 each, so 9.1e-7 of tanh);
+* GELU: 2.5e-7 absolute and half a step of f32 (the fit is off by 8e-8, the polynomial's f32 steps and the exponential by
+  1.3e-7 together), and for negative arguments also relative: 1e-3 down to -5.5, 8e-3 below (the fit of log2 Phi is off by
+  8e-4 and 6e-3 of Phi), down to f32's least normal number, below which the exponential is 0."""
+import math
+
 import numpy as np
 import pytest
 
@@ -14,6 +19,8 @@ pytestmark = pytest.mark.gpu
 from ancha_b200 import microscaled as mx  # noqa: E402
 from oracle import microscaled as O  # noqa: E402
 from test_gpu_microscaled import FORMATS, check_near, f64, poisoned_memory, rows_of, scalar  # noqa: E402,F401
+
+LEAST = 2.0 ** -126  # f32's least normal number
 
 
 # ---------------------------------------------------------------------------------------- norm
@@ -48,14 +55,23 @@ def sums(m, top):
     return x, mx.quantize(torch.eye(k, device="cuda"), "mxf8"), f64(mx.dequantize(x))
 
 
+def gelu64(z):
+    return np.vectorize(lambda t: 0.5 * t * math.erfc(-t / math.sqrt(2)))(z)
+
+
 def activation(act, z):
     """(activation, tolerance) in float64."""
-    y = np.tanh(z)
-    return y, 1e-6 * np.abs(y)
+    if act == "tanh":
+        y = np.tanh(z)
+        return y, 1e-6 * np.abs(y)
+    y = gelu64(z)
+    tol = 2.5e-7 + 2.0 ** -24 * np.abs(y)
+    rel = np.where(z < -5.5, 8e-3, 1e-3)
+    return y, np.where(z < 0, np.minimum(tol, rel * np.abs(y) + 16 * LEAST), tol)
 
 
 @pytest.mark.parametrize("m", [3, 40, 300])
-@pytest.mark.parametrize("act", ["tanh"])
+@pytest.mark.parametrize("act", ["tanh", "gelu"])
 @pytest.mark.parametrize("top", [4.0, 0.05])
 def test_activations_over_their_range(m, act, top):
     x, w, z = sums(m, top)
@@ -72,3 +88,32 @@ def test_small_tanh_keeps_its_blocks(m, fmt):
     y, tol = activation("tanh", z)
     g = 2.0 ** -30 if fmt == "nvf4" else None
     check_near(mx.linear(x, w, None, "tanh", format=fmt, global_scale=scalar(g)), y, tol)
+
+
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lo,hi", [(-5.5, -4.0), (-7.0, -5.6), (-12.5, -9.0), (-6.0, -5.0), (-3e4, -20.0)])
+def test_gelu_of_negative_sums_keeps_its_blocks(m, fmt, lo, hi):
+    """Blocks of sums so negative that GELU is next to nothing: their scale and codes are those of what is left."""
+    k = 256
+    v = np.random.default_rng(m).uniform(lo, hi, (m, k))
+    x = mx.quantize(torch.from_numpy(v).float().cuda(), "mxf8")
+    z = f64(mx.dequantize(x))
+    y, tol = activation("gelu", z)
+    w = mx.quantize(torch.eye(k, device="cuda"), "mxf8")
+    got = f64(mx.linear(x, w, None, "gelu", dtype=torch.float32))
+    assert (np.abs(got - y) <= tol).all(), float((np.abs(got - y) / tol).max())
+    g = max(np.abs(y).max() / (6 * 448), 2.0 ** -120) if fmt == "nvf4" else None
+    check_near(mx.linear(x, w, None, "gelu", format=fmt, global_scale=scalar(g)), y, tol)
+
+
+def test_gelu_does_not_depend_on_its_neighbours():
+    """The same sums give the same bits beside very negative ones and without them."""
+    k, m = 256, 300
+    v = torch.from_numpy(np.random.default_rng(7).uniform(-5.4, 9, (m, k))).float().cuda()
+    far = v.clone()
+    far[:, ::64] = -7.0
+    w = mx.quantize(torch.eye(k, device="cuda"), "mxf8")
+    a, b = (mx.linear(mx.quantize(t, "mxf8"), w, None, "gelu", dtype=torch.float32) for t in (v, far))
+    same = mx.dequantize(mx.quantize(v, "mxf8")) == mx.dequantize(mx.quantize(far, "mxf8"))
+    assert same.float().mean() > 0.9 and torch.equal(a[same], b[same])
