@@ -19,6 +19,7 @@
 #include "tc.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace ancha {
 namespace {
@@ -217,6 +218,18 @@ __device__ __forceinline__ void add8(const uint4& q, int type, float (&v)[32], i
         v[j + 2 * i] += f.x;
         v[j + 2 * i + 1] += f.y;
     }
+}
+
+// The product of the arrays' scales, which the sums are multiplied by. It may leave f32's normal numbers where the sums times it
+// do not: then a power of two of it, `pre`, goes to the sums first. (Sums are 0 or between 2^-20 and 2^54, so neither step
+// loses what the result holds; above 2^192 the factor is f32's largest number, which leaves 0 at 0 and overflows all else.)
+__device__ __forceinline__ float array_scale(const Params& p, float& pre) {
+    const float gx = p.gx ? *p.gx : 1.f, gw = p.gw ? *p.gw : 1.f, g = gx * gw;
+    pre = 1.f;
+    if (g >= FLT_MIN && g <= FLT_MAX) return g;
+    pre = g < 1.f ? 0x1p-64f : 0x1p64f;
+    const double r = (double)gx * gw / pre;
+    return r > FLT_MAX ? FLT_MAX : (float)r;  // NaN stays
 }
 
 // act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them). `bias`: theirs, in shared
@@ -588,7 +601,8 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
         uint64_t* rbar = &rfull[warp - 2];
         float* bias = reinterpret_cast<float*>(biases) + (warp - 2) * 64;
         float alpha = 1.f;
-        if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
+        float pre = 1.f;
+        if (FMT == NVF4) alpha = array_scale(p, pre);
         const bool wide = p.out_mode == OUT_TMA && p.out_type == ELT_F32;
         float b0 = 0.f, b1 = 0.f;
         const auto load_bias = [&](int ni) {
@@ -636,6 +650,10 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
                 if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0));
                 else mbar_arrive(bar);
+            }
+            if (FMT == NVF4 && pre != 1.f) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) r[j / 32][j % 32] = __float_as_uint(__uint_as_float(r[j / 32][j % 32]) * pre);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -876,7 +894,8 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
         tmem_dealloc(tmem, S::COLS);
     }
     float alpha = 1.f;
-    if (FMT == NVF4) alpha = (p.gx ? *p.gx : 1.f) * (p.gw ? *p.gw : 1.f);
+    float pre = 1.f;
+    if (FMT == NVF4) alpha = array_scale(p, pre);
     const int col = n0 + 4 * lane, nv = min(4, p.n - col);  // this lane's columns
     float bias[4] = {};
     if (p.bias) {
@@ -895,7 +914,7 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
             v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = fmaf(v[j], alpha, bias[j]);
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(FMT == NVF4 ? v[j] * pre : v[j], alpha, bias[j]);
         if (p.act == ANCHA_ACT_GELU) {
             gelu2(v[0], v[1]);
             gelu2(v[2], v[3]);

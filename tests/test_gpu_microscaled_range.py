@@ -117,3 +117,33 @@ def test_gelu_does_not_depend_on_its_neighbours():
     a, b = (mx.linear(mx.quantize(t, "mxf8"), w, None, "gelu", dtype=torch.float32) for t in (v, far))
     same = mx.dequantize(mx.quantize(v, "mxf8")) == mx.dequantize(mx.quantize(far, "mxf8"))
     assert same.float().mean() > 0.9 and torch.equal(a[same], b[same])
+
+
+# -------------------------------------------------------------------------------- array scales
+
+@pytest.mark.parametrize("m", [3, 300])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gx,gw,size", [(3e-22, 5e-22, 1.0), (7e-20, 2e-25, 1.0), (1e-30, 1e-30, 1.0), (2e30, 1e9, 2.0 ** -7),
+                                        (1e30, 1e-31, 1.0)])
+def test_products_of_extreme_array_scales(m, out, gx, gw, size):
+    """Array scales whose product leaves f32's normal numbers: the products of the arrays need not."""
+    n, k = 200, 96
+
+    def operand(rows, seed):  # an array without an array scale, whose row 1 holds zeros
+        v = np.random.default_rng(seed).standard_normal((rows, k)) * (2000 if size == 1.0 else size)
+        v[1] = 0
+        return mx.quantize(torch.from_numpy(v).float().cuda(), "nvf4")
+
+    x, w = operand(m, 1), operand(n, 2)
+    a, b = f64(mx.dequantize(x)), f64(mx.dequantize(w))
+    x.global_scale, w.global_scale = scalar(gx), scalar(gw)
+    g = float(np.float32(gx)) * float(np.float32(gw))
+    y, mass = (a @ b.T) * g, (np.abs(a) @ np.abs(b).T) * g
+    top = float(torch.finfo(out).max)
+    got = f64(mx.linear(x, w, dtype=out))
+    assert np.isfinite(got[np.abs(y) < top * 0.99]).all() and not got[1].any()
+    ok = np.isfinite(got)
+    assert ok.mean() > 0.9
+    # Sum and product as ever; what is below f32's least normal number rounds to its subnormal step.
+    tol = (k + 4) * 2.0 ** -23 * mass + (0 if out == torch.float32 else 2.0 ** -8) * np.abs(y) + 2.0 ** -132
+    assert (np.abs(got - y)[ok] <= tol[ok]).all()
