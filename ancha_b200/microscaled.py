@@ -181,7 +181,7 @@ def _run(device: int, fn, *args):
 def quantize(x: torch.Tensor, format: str = "mxf8", global_scale: Optional[torch.Tensor] = None) -> Microscaled:
     """Quantise the rows of ``x [rows, cols]`` (f32, bf16 or f16; any row stride). Scales and rounding as
     ``ancha_mx_quantize`` says. ``global_scale`` (``nvf4``): one f32 on the device, usually
-    ``max|x| / (6 * 448)``; it becomes the array's."""
+    ``max|x| / (6 * 448)`` and at most 2^125; it becomes the array's."""
     device = _device(x)
     dtype, ld = _matrix(x, device, "x")
     rows, cols = x.shape

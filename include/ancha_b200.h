@@ -180,8 +180,9 @@ enum { ANCHA_MXF8 = 0, ANCHA_MXF4 = 1, ANCHA_NVF4 = 2 };
  * Calls that write an array write the element bytes of a row up to the next multiple of 16 and every
  * byte of the scale tiles, with zeros behind the last column, row and block; data behind that, and rows
  * behind `rows`, are left as they were. Calls that read one need the scales behind a row's last block to
- * be numbers (not NaN: zeros) and, with an odd number of 4-bit columns, the other half of the last byte 0. `global_scale`: the array scale, one device f32 > 0, or NULL for 1;
- * ANCHA_NVF4 only. */
+ * be numbers (not NaN: zeros) and, with an odd number of 4-bit columns, the other half of the last byte 0.
+ * `global_scale`: the array scale, one device f32 from 2^-149 to 2^125 (so that six of it are an f32 number; 0 with an
+ * array of zeros), or NULL for 1; ANCHA_NVF4 only. */
 typedef struct {
     int format;
     int64_t rows, cols;        /* rows >= 0, 1 <= cols < 2^31 - 512 */

@@ -147,3 +147,25 @@ def test_products_of_extreme_array_scales(m, out, gx, gw, size):
     # Sum and product as ever; what is below f32's least normal number rounds to its subnormal step.
     tol = (k + 4) * 2.0 ** -23 * mass + (0 if out == torch.float32 else 2.0 ** -8) * np.abs(y) + 2.0 ** -132
     assert (np.abs(got - y)[ok] <= tol[ok]).all()
+
+
+@pytest.mark.parametrize("g", [2.0 ** -149, 1e-38, 5e37, 2.0 ** 125])
+def test_quantisation_with_the_ends_of_the_array_scale(g):
+    """The least number of f32, and the largest of which six are one."""
+    x = torch.clamp(rows_of(20, 200, torch.float32, 1, 0), -3, 3) * (1e38 if g > 1 else 1e-37)
+    x[3] = 0
+    q = mx.quantize(x, "nvf4", scalar(g))
+    check_near(q, f64(x), 2.0 ** -22 * np.abs(f64(x)) + 2.0 ** -149)
+    assert f64(mx.dequantize(q)).any()
+
+
+@pytest.mark.parametrize("m", [3, 300])
+def test_zeros_with_the_array_scale_of_zeros(m):
+    """max|x| / (6 * 448) of an array of zeros is 0: the array and its products are zeros."""
+    x, v = torch.zeros((m, 200), device="cuda"), rows_of(130, 200, torch.float32, 2)
+    q, w = mx.quantize(x, "nvf4", x.abs().max().view(1) / (6 * 448)), mx.quantize(v, "nvf4", scalar(0.001))
+    assert not mx.dequantize(q).any() and not mx.linear(q, w).any() and not mx.linear(w, q).any()
+    s, _ = mx.add_rms_norm(x, None, None, format="nvf4", global_scale=q.global_scale)
+    assert not mx.dequantize(s).any() and not mx.linear(s, w).any()
+    y = mx.linear(q, w, format="nvf4", global_scale=q.global_scale)
+    assert not mx.dequantize(y).any()
