@@ -206,7 +206,7 @@ def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tens
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, gain: Optional[torch.Tensor] = None,
                  eps: float = 1e-6, format: str = "mxf8", global_scale: Optional[torch.Tensor] = None,
                  residual_out: Optional[torch.Tensor] = None):
-    """``s = residual + x`` (``x`` without a residual), and the quantised rows of
+    """``s = residual + x`` (``x`` without a residual), added in f32 and rounded to the residual's dtype, and the quantised rows of
     ``s / sqrt(mean(s^2) + eps) * gain``. Returns ``(Microscaled, s)``; ``s`` has the residual's dtype and
     is ``x`` itself without a residual. ``residual_out`` takes ``s`` (``residual`` itself: in place).
     ``x`` and ``residual``: f32, bf16 or f16 ``[rows, cols]``, at most 32768 columns; ``gain``: f32 ``[cols]``."""

@@ -215,7 +215,8 @@ typedef struct {
     double eps;                   /* > 0                                                       */
 } ancha_mx_norm_desc;
 
-/* s = residual + x, rounded to residual_dtype and written to residual_out; out = the quantised rows of
+/* s = residual + x, added in f32, rounded to residual_dtype and written to residual_out (with an f32 x and a 16-bit
+ * residual the sum is rounded twice, which can differ from once next to a tie); out = the quantised rows of
  * s / sqrt(mean(s^2) + eps) * gain. `residual` NULL: s = x (then residual_dtype = dtype), written to
  * residual_out unless that is NULL too. gain: device f32 [cols] or NULL for 1. residual_out may be
  * residual or x itself, with the same row stride and type; any other overlap is undefined. Rows of at most

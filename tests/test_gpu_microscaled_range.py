@@ -169,3 +169,19 @@ def test_zeros_with_the_array_scale_of_zeros(m):
     assert not mx.dequantize(s).any() and not mx.linear(s, w).any()
     y = mx.linear(q, w, format="nvf4", global_scale=q.global_scale)
     assert not mx.dequantize(y).any()
+
+
+# --------------------------------------------------------------------------- rounding of the stream
+
+@pytest.mark.parametrize("kind,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_the_stream_is_added_in_f32_and_then_rounded(kind, half):
+    """A sum just above a tie of the stream's type, by less than f32 holds: the f32 sum is the tie, which goes to
+    the even number. A sum of two 16-bit numbers that f32 does not hold is never next to a tie."""
+    x = torch.full((2, 64), half, device="cuda")
+    x[:, 1::2] *= 1 + 2.0 ** -20
+    r = torch.ones((2, 64), dtype=kind, device="cuda")
+    _, s = mx.add_rms_norm(x, r)
+    assert s.dtype == kind and (s == 1).all()
+    x[:, 0::2] *= 1 + 2.0 ** -10  # f32 holds this one
+    _, s = mx.add_rms_norm(x, r)
+    assert (s[:, 0::2].double() == 1 + 2 * half).all() and (s[:, 1::2] == 1).all()
