@@ -426,6 +426,28 @@ __device__ __forceinline__ uint32_t stage_mx(const MxArray& o, uint8_t* buf, int
     return codes;
 }
 
+// Behind a wait that gave up, with every warp past its last issue: what the CTA has in flight ends before its shared memory and
+// TMEM are given back (each bounded again). load_drain: the copies of the last `stages` of `issued` slabs, by one thread;
+// product_drain: the products, by a converged warp whose commit on `bar`, unused so far, follows them.
+__device__ void load_drain(uint64_t* full, uint32_t stages, uint32_t issued) {
+    const long long c0 = clock64();
+    for (uint32_t j = issued > stages ? issued - stages : 0; j < issued; ++j)
+        while (!mbar_try_wait(&full[j % stages], (j / stages) & 1) && clock64() - c0 < kWaitCycles) {
+        }
+}
+template <bool PAIR>
+__device__ __forceinline__ void product_drain(uint64_t* bar) {
+    if (elect_one()) {
+        if (PAIR) umma_commit_pair(bar, 0x1);
+        else umma_commit(bar);
+    }
+    __syncwarp();
+    const long long c0 = clock64();
+    while (!mbar_try_wait(bar, 0) && clock64() - c0 < kWaitCycles) {
+    }
+    __syncwarp();
+}
+
 // A converged warp's wait; false where one lane's ran out.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;  // no clock read where there is no wait
@@ -472,8 +494,10 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     uint64_t* tfull = empty + stages;   // [2] accumulator ready
     uint64_t* tempty = tfull + 2;       // [2] accumulator drained (with shared columns: [0], those drained)
     uint64_t* rfull = tempty + 2;       // [EPI] residual arrived
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rfull + EPI);
+    uint64_t* drain = rfull + EPI;      // used behind an abort alone
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile uint32_t* issued = tmem_slot + 2;  // slabs loaded
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -489,6 +513,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             mbar_init(&tempty[b], PAIR ? 2 * EPI : EPI);
         }
         for (int w = 0; w < EPI; ++w) mbar_init(&rfull[w], 1);
+        mbar_init(drain, 1);
         *abort = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -549,13 +574,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
                 }
             }
         }
-        if (*abort && rank == 0 && lane == 0) {  // let copies in flight land before the CTA exits (bounded)
-            const long long c0 = clock64();
-            for (uint32_t j = it > (uint32_t)stages ? it - stages : 0; j < it; ++j)
-                while (!mbar_try_wait(&full[j % stages], (j / stages) & 1) && clock64() - c0 < kWaitCycles) {
-                }
-        }
-        __syncwarp();
+        if (lane == 0) *issued = it;
     } else if (warp == 1) {
         if (rank == 0) {
             constexpr uint32_t idesc = idesc_of<FMT>(BMT, BN);
@@ -726,6 +745,11 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort && rank == 0) {  // the even CTA's barriers count the odd one's copies too
+        if (threadIdx.x == 0) load_drain(full, stages, *issued);
+        if (warp == 1) product_drain<PAIR>(drain);
+        __syncthreads();
+    }
     // With a pair, neither CTA releases TMEM or exits while the other may still use its shared memory.
     if (PAIR) cluster_sync();
     if (warp == 1) {
@@ -802,8 +826,10 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
     uint64_t* full = reinterpret_cast<uint64_t*>(sx_tiles + STAGES * S::SF * SF_TILE);
     uint64_t* empty = full + STAGES;
     uint64_t* done = empty + STAGES;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* drain = done + 1;  // used behind an abort alone
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile uint32_t* issued = tmem_slot + 2;  // slabs loaded
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = (int)blockIdx.x % splits, n0 = (int)blockIdx.x / splits * BM, m0 = (int)blockIdx.y * TN;
@@ -813,6 +839,7 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
             mbar_init(&empty[s], 1);
         }
         mbar_init(done, 1);
+        mbar_init(drain, 1);
         *abort = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -846,13 +873,7 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
             }
             __syncwarp();
         }
-        if (*abort && lane == 0) {  // let copies in flight land before the CTA exits (bounded)
-            const long long c0 = clock64();
-            for (uint32_t j = it > (uint32_t)STAGES ? it - STAGES : 0; j < it; ++j)
-                while (!mbar_try_wait(&full[j % STAGES], (j / STAGES) & 1) && clock64() - c0 < kWaitCycles) {
-                }
-        }
-        __syncwarp();
+        if (lane == 0) *issued = it;
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_of<FMT>(BM, TN);
         uint32_t it = 0;
@@ -884,12 +905,15 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
 #pragma unroll
                 for (int j = 0; j < 16; ++j) partial[(c + j) * BM + quarter * 32 + lane] = __uint_as_float(r[j]);
             }
+        } else {  // the sums are missing, which the peers' results show
+            for (int c = 0; c < live; ++c) partial[c * BM + quarter * 32 + lane] = __int_as_float(0x7FC00000);
         }
         tc_fence_before();
     }
     __syncwarp();
     cluster_sync();
     if (warp == 1) {
+        if (*abort) product_drain<false>(drain);
         tc_fence_after();
         tmem_dealloc(tmem, S::COLS);
     }
@@ -937,6 +961,10 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
         for (int64_t i = rank * SPLIT_THREADS + threadIdx.x; i < (end - p.m) * words; i += splits * SPLIT_THREADS)
             *reinterpret_cast<uint32_t*>(p.om.scales + mx_scale_word(p.m + i / words, n0 / (4 * b) + (int)(i % words), p.okt)) = 0;
     }
+    __syncwarp();
+    if (*abort && threadIdx.x == 0) load_drain(full, STAGES, *issued);
+    __syncwarp();
+    if (*abort && threadIdx.x == 0) load_drain(full, STAGES, *issued);
     __syncwarp();
     cluster_sync();  // a CTA's shared memory stays while its peers read it
 }
