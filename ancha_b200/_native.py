@@ -25,7 +25,8 @@ STATUS_NAMES = {OK: "ok", E_UNSUPPORTED: "unsupported", E_INVALID: "invalid", E_
                 E_NONFINITE: "non-finite"}
 
 # Every symbol the header declares (checked by the CPU test suite).
-EXPORTS = ("ancha_last_error", "ancha_version", "ancha_available", "ancha_wait_selftest", "ancha_attention_fwd",
+EXPORTS = ("ancha_last_error", "ancha_version", "ancha_available", "ancha_wait_selftest", "ancha_wait_selftest_launch",
+           "ancha_device_error", "ancha_attention_fwd",
            "ancha_attention_workspace", "ancha_attention_fwd_ws", "ancha_linear_fwd", "ancha_linear_workspace",
            "ancha_linear_fwd_ws", "ancha_mx_layout", "ancha_mx_quantize", "ancha_mx_dequantize",
            "ancha_mx_add_rms_norm_fwd", "ancha_mx_linear_fwd", "ancha_stft_fwd", "ancha_istft_masked", "ancha_istft_masked_static", "ancha_ola_add",
@@ -116,6 +117,8 @@ def lib() -> C.CDLL:
             "ancha_version": (C.c_char_p, []),
             "ancha_available": (i32, [i32]),
             "ancha_wait_selftest": (i32, [i64, vp]),
+            "ancha_wait_selftest_launch": (i32, [i64, vp]),
+            "ancha_device_error": (i32, [vp]),
             "ancha_attention_fwd": (i32, [C.POINTER(AttnDesc), vp, vp, vp, vp, vp, vp]),
             "ancha_attention_workspace": (i32, [C.POINTER(AttnDesc), C.POINTER(C.c_size_t)]),
             "ancha_attention_fwd_ws": (i32, [C.POINTER(AttnDesc), vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),

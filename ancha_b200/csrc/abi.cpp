@@ -136,8 +136,14 @@ const char* ancha_last_error(void) { return g_last_error.c_str(); }
 const char* ancha_version(void) { return "ancha-b200 0.1.0 (sm_100a)"; }
 
 int ancha_wait_selftest(int64_t budget_cycles, void* stream) {
-    return wait_selftest((long long)budget_cycles, as_stream(stream));
+    return wait_selftest((long long)budget_cycles, false, as_stream(stream));
 }
+
+int ancha_wait_selftest_launch(int64_t budget_cycles, void* stream) {
+    return wait_selftest((long long)budget_cycles, true, as_stream(stream));
+}
+
+int ancha_device_error(void* stream) { return take_device_error(as_stream(stream)); }
 
 int ancha_available(int device) {
     int count = 0;

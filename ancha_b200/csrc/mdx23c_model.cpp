@@ -20,6 +20,7 @@
 #include <thread>
 
 #include "gemm.cuh"
+#include "tc.cuh"
 
 namespace ancha {
 
@@ -581,7 +582,7 @@ int Mdx23c::separate_pcm(const float* planes, int64_t samples, int overlap, int 
         ANCHA_CUDA(cudaMemcpyAsync(stems, sums.p, sums.bytes, cudaMemcpyDeviceToHost, s));
         int status = 0;
         ANCHA_CUDA(cudaMemcpyAsync(&status, flag.p, sizeof(int), cudaMemcpyDeviceToHost, s));
-        ANCHA_CUDA(cudaStreamSynchronize(s));
+        ANCHA_TRY(take_device_error(s));  // synchronises the stream
         if (status & 1) return fail(ANCHA_E_NONFINITE, "non-finite MDX23C output");
         if (status & 2) return fail(ANCHA_E_INVALID, "iSTFT has an uncovered sample");
     } catch (const std::exception& e) {

@@ -9,6 +9,7 @@
 
 #include "mdx_exec.hpp"
 #include "rowops.cuh"
+#include "tc.cuh"
 
 namespace ancha {
 namespace {
@@ -503,7 +504,7 @@ int MdxModel::separate_pcm(const MdxTaskOpts& o, const float* planes, int64_t sa
         ANCHA_CUDA(cudaMemcpyAsync(residual, res.p, res.bytes, cudaMemcpyDeviceToHost, s));
         int status = 0;
         ANCHA_CUDA(cudaMemcpyAsync(&status, flag.p, sizeof(int), cudaMemcpyDeviceToHost, s));
-        ANCHA_CUDA(cudaStreamSynchronize(s));
+        ANCHA_TRY(take_device_error(s));  // synchronises the stream
         if (status & 1) return fail(ANCHA_E_NONFINITE, "non-finite MDX output");
         if (status & 2) return fail(ANCHA_E_INVALID, "MDX OLA uncovered sample; overlap setting is invalid");
     } catch (const std::exception& e) {

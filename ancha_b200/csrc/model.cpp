@@ -20,6 +20,7 @@
 #include "attention.cuh"
 #include "dsp.cuh"
 #include "rowops.cuh"
+#include "tc.cuh"
 
 #ifndef ANCHA_FP32_SPLIT
 #define ANCHA_FP32_SPLIT 1
@@ -787,8 +788,7 @@ int Model::read_flag(cudaStream_t s, int* flag) {
     *flag = 0;
     if (!flag_.p) return ANCHA_OK;
     ANCHA_CUDA(cudaMemcpyAsync(flag, flag_.p, sizeof(int), cudaMemcpyDeviceToHost, s));
-    ANCHA_CUDA(cudaStreamSynchronize(s));
-    return ANCHA_OK;
+    return take_device_error(s);
 }
 
 int Model::forward(const float* spectrum, int chunks, int frames, float* masks,

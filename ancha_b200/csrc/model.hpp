@@ -104,7 +104,7 @@ public:
     int forward(const float* spectrum, int chunks, int frames, float* masks,
                 const volatile int* cancel, cudaStream_t stream, bool check = true);
     int reset_flag(cudaStream_t s);
-    int read_flag(cudaStream_t s, int* flag);  // synchronises `s`
+    int read_flag(cudaStream_t s, int* flag);  // synchronises `s`; fails where a device-side wait gave up
 
     PipelineBuffers pipe;
 

@@ -4,7 +4,8 @@
 //
 // Every wait is bounded by a clock budget: on expiry the thread raises the CTA's abort flag
 // and ORs ANCHA_DEVICE_TIMEOUT into the library's device error word, and every loop of the
-// kernel unwinds, so a lost arrival ends the kernel with an error status instead of hanging.
+// kernel unwinds, so a lost arrival ends the kernel, its output unfinished, instead of hanging. The
+// host reads the word at its synchronisation points and in ancha_device_error (take_device_error).
 #pragma once
 
 #include <cuda.h>
@@ -17,15 +18,16 @@ constexpr int ANCHA_DEVICE_TIMEOUT = 1;
 // ~1 s at the B200 boost clock.
 constexpr long long kWaitCycles = 2000000000ll;
 
-// Device error word of this device (allocated on first use, zero = no error).
+// Device error word of this device (zero = no error).
 int* device_error_word();
 // Read and clear the device error word (synchronises `s`); ANCHA_E_TIMEOUT if it was set.
 int take_device_error(cudaStream_t s);
 
 // Watchdog self-test: one CTA waits, with a budget of `budget_cycles`, on an mbarrier that
 // nothing arrives at, through the same bounded wait as the tensor-core kernels; returns the
-// status the host reads back (ANCHA_E_TIMEOUT when the watchdog works).
-int wait_selftest(long long budget_cycles, cudaStream_t s);
+// status the host reads back (ANCHA_E_TIMEOUT when the watchdog works). With `record` the timeout goes
+// to the device error word, as a kernel's does, and the call only launches.
+int wait_selftest(long long budget_cycles, bool record, cudaStream_t s);
 
 // Encode a 3-D tiled tensor map over a row-major [depth][rows][cols] array of 2-byte
 // elements (row stride `ld`, depth stride `depth_stride`, in elements) with a

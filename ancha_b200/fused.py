@@ -31,6 +31,15 @@ def available(device: int = 0) -> bool:
         return False
 
 
+def check_device(device=None) -> None:
+    """Wait for torch's current stream of ``device`` (default: the current one) and raise ``AnchaError``
+    (timeout) if a kernel of this library has given up a device-side wait there since it was last asked. The
+    kernels of this module and of ``microscaled`` are only enqueued, so nothing else reports that."""
+    torch = _torch()
+    with torch.cuda.device(device):
+        N.check(N.lib().ancha_device_error(_stream()))
+
+
 def _dtype_code(t) -> int:
     torch = _torch()
     if t.dtype == torch.float32:

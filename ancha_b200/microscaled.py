@@ -17,7 +17,8 @@ tensor cores (``fused.linear`` is the 16-bit and 32-bit form). A pre-norm feed-f
 
 The functions run on the stream that is torch's current one on the tensors' device, allocate only what
 they return, keep nothing between calls and never synchronise, so they can be captured into CUDA graphs.
-They raise ``AnchaError`` for arguments they do not take. No gradients: this is an inference engine.
+They raise ``AnchaError`` for arguments they do not take; ``fused.check_device`` raises it where a kernel has
+given up a device-side wait. No gradients: this is an inference engine.
 """
 from __future__ import annotations
 

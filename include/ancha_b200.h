@@ -64,11 +64,23 @@ ANCHA_API int ancha_available(int device);
 /* Watchdog self-test of the current device: one kernel waits, with a budget of `budget_cycles`
  * SM clock cycles (0 to the kernels' own ~1 s budget), on an mbarrier that nothing arrives at,
  * through the same bounded wait every tensor-core kernel uses; the kernel gives up, records the
- * timeout in the library's device error word and returns. Returns ANCHA_E_TIMEOUT (with a
- * message) when the watchdog works; the device stays usable and the error word is cleared.
+ * timeout in a word of its own and returns. Returns ANCHA_E_TIMEOUT (with a message) when the
+ * watchdog works; the device stays usable, and what ancha_device_error reports is left alone.
  * Diagnostics of the failure path that src/device.rs:11-41 and tests/cuda_device_failure.rs
  * cover in the reference; synchronises `stream`. */
 ANCHA_API int ancha_wait_selftest(int64_t budget_cycles, void* stream);
+
+/* The self-test's kernel alone, enqueued on `stream`: its timeout goes to the library's device error
+ * word, as that of any kernel whose wait gives up, and ancha_device_error then reports it. */
+ANCHA_API int ancha_wait_selftest_launch(int64_t budget_cycles, void* stream);
+
+/* Kernels with device-side waits give up after about a second, record that in the device error word and end
+ * with their output unfinished or NaN; calls that only enqueue have returned ANCHA_OK by then. Synchronises
+ * `stream` and returns ANCHA_E_TIMEOUT, clearing the word, if a kernel of this library has given up on
+ * the current device since it was last cleared, else ANCHA_OK. The word is the device's: of several
+ * callers one is told. Calls that synchronise themselves (ancha_model_forward, the separations,
+ * ancha_separate_status) read it too. Not during stream capture. */
+ANCHA_API int ancha_device_error(void* stream);
 
 /* ------------------------------------------------------------------------------------ *
  * Kernel plug-in API (replaces crates/ancha-models/src/fused/mod.rs)                   *
