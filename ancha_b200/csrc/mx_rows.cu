@@ -332,7 +332,6 @@ template <int FMT, int W, int CH>
 __global__ void __launch_bounds__(W > 8 ? 32 * W : 256, W > 8 ? 1 : W == 8 ? 6 : W == 1 ? 4 : 5)
 add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
     constexpr int THREADS = W > 8 ? 32 * W : 256, ROWS = THREADS / (32 * W);
-    constexpr int AHEAD = CH <= 2 ? CH : 1;  // chunks of the residual on their way at once
     __shared__ double part[THREADS / 32];
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / (32 * W);
     const int t = threadIdx.x % (32 * W), warp = threadIdx.x / 32;
@@ -350,19 +349,15 @@ add_rms_norm_kernel(const __grid_constant__ NormArgs a) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) fetch16<32>(x, a.dtype, a.access, (t + i * 32 * W) * PER, n, v[i]);
         if (a.residual) {
-            float u[AHEAD][PER];
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                if (i % AHEAD == 0) {
-#pragma unroll
-                    for (int k = 0; k < AHEAD; ++k)
-                        fetch16<32>(r, a.res_type, a.access_r, (t + (i + k) * 32 * W) * PER, n, u[k]);
-                }
+                float u[PER];
+                fetch16<32>(r, a.res_type, a.access_r, (t + i * 32 * W) * PER, n, u);
                 settle16<32>(a.access, buf, v[i]);
-                settle16<32>(a.access_r, buf, u[i % AHEAD]);
+                settle16<32>(a.access_r, buf, u);
 #pragma unroll
                 for (int j = 0; j < PER; j += 2)
-                    f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[i % AHEAD][j], u[i % AHEAD][j + 1])), v[i][j], v[i][j + 1]);
+                    f2_split(fadd2(f2(v[i][j], v[i][j + 1]), f2(u[j], u[j + 1])), v[i][j], v[i][j + 1]);
             }
         } else {
 #pragma unroll
