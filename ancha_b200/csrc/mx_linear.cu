@@ -29,7 +29,7 @@ constexpr int OPERAND_BYTES = BM * SLAB;     // 128 rows of a slab
 constexpr int SF_TILE = 512;                 // a scale tile
 constexpr int STAGING = 4096;                // per epilogue warp: 32 rows x 128 bytes
 constexpr int BIAS_BYTES = 256;              // and the bias of its 64 columns
-// TMEM: two accumulators, then the scales of the slab in work.
+// TMEM: one accumulator or two, then the scales of the slab in work.
 constexpr uint32_t SFA_COL = 448, SFB_COL = 464, TMEM_COLS = 512;
 
 constexpr int sf_tiles(int fmt) { return fmt == MXF8 ? 1 : fmt == MXF4 ? 2 : 4; }
@@ -54,10 +54,9 @@ struct Shape {
         return FIXED + (residual ? EPI * STAGING : 0) + stages(residual) * STAGE;
     }
     static_assert(stages(true) >= 2, "shared memory");
-    // Second accumulator. Two of 256 columns and the scales do not fit 512: they share 64 columns, which
-    // the epilogue of a tile drains first, so the next tile's products start when those are free.
-    static constexpr uint32_t ACC1 = BN == 256 ? 192 : BN;
-    static constexpr bool SHARED_COLS = BN == 256;
+    // Accumulators, used in turn. Two of 256 columns and the scales do not fit TMEM's 512: with one, a tile's products
+    // start when every epilogue warp has read the tile before into registers.
+    static constexpr int ACCS = BN == 256 ? 1 : 2;
 };
 
 struct Params {
@@ -492,7 +491,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + stages * S::SFB_BYTES);
     uint64_t* empty = full + stages;
     uint64_t* tfull = empty + stages;   // [2] accumulator ready
-    uint64_t* tempty = tfull + 2;       // [2] accumulator drained (with shared columns: [0], those drained)
+    uint64_t* tempty = tfull + 2;       // [2] accumulator drained
     uint64_t* rfull = tempty + 2;       // [EPI] residual arrived
     uint64_t* drain = rfull + EPI;      // used behind an abort alone
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -581,14 +580,10 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             int s = 0;
             uint32_t phase = 0, local = 0;
             for (int t = tile0; t < p.tiles && !*abort; t += tstep, ++local, walk.next()) {
-                const int b = local & 1;
-                if (S::SHARED_COLS) {
-                    if (local && !warp_wait(&tempty[0], (local - 1) & 1, abort, p.err)) break;
-                } else if (!warp_wait(&tempty[b], ((local >> 1) & 1) ^ 1, abort, p.err)) {
-                    break;
-                }
+                const uint32_t b = local % S::ACCS;
+                if (!warp_wait(&tempty[b], (local / S::ACCS & 1) ^ 1, abort, p.err)) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + b * S::ACC1;
+                const uint32_t acc = tmem + b * BN;
                 for (int kb = 0; kb < slabs; ++kb) {
                     if (!warp_wait(&full[s], phase, abort, p.err)) break;
                     tc_fence_after();
@@ -644,7 +639,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
         };
         uint32_t local = 0;
         for (int t = tile0; t < p.tiles; t += tstep, ++local) {
-            const int c_first = walk.ni * BN + col0, b = local & 1;
+            const int c_first = walk.ni * BN + col0, b = local % S::ACCS;
             const int64_t row0 = (int64_t)walk.mi * BMT + (int)rank * BM + quarter * 32, row = row0 + lane;
             const bool some = row0 < p.m && c_first < p.n;
             walk.next();
@@ -654,9 +649,9 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             bias[32 + lane] = b1;
             if (p.bias && t + tstep < p.tiles) load_bias(walk.ni);
             if (RES && res_tma && some) load_res(c_first, row0);
-            if (!warp_wait(&tfull[b], (local >> 1) & 1, abort, p.err)) break;
+            if (!warp_wait(&tfull[b], local / S::ACCS & 1, abort, p.err)) break;
             tc_fence_after();
-            const uint32_t base = tmem + b * S::ACC1 + col0 + ((uint32_t)(quarter * 32) << 16);
+            const uint32_t base = tmem + b * BN + col0 + ((uint32_t)(quarter * 32) << 16);
             bool res_ok = true;
             uint32_t codes = 0, r[2][32];
             tmem_ld32(base, r[0]);
@@ -666,7 +661,7 @@ linear_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                uint64_t* bar = &tempty[S::SHARED_COLS ? 0 : b];
+                uint64_t* bar = &tempty[b];
                 if (PAIR) mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0));
                 else mbar_arrive(bar);
             }
