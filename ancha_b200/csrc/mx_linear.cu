@@ -12,9 +12,10 @@
 // columns each). A CTA pair shares a tile of 256 rows by 192 or 256 columns (each CTA holds 128 rows of x, half of w's rows,
 // and all of w's scales). Few rows, or few tiles with long K, take the split kernel at the end.
 //
-// Measured (one B200): 8192^3 nvf4 233 us = 4.7 PFLOP/s, mxf4 200 us = 5.5, mxf8 437 us = 2.5 under the power cap, where the
-// tensor pipe and the scale copies are the limit (a slab's 512 cycles of products and 3, 6 or 12 copies); 48060 x 1536 x 384
-// mxf8 with GELU into mxf8 72 us, where the epilogue's arithmetic is (44 us without GELU); 1 x 4096 x 4096 mxf4 7 us, latency.
+// Measured (one B200): 8192^3 nvf4 229 us = 4.8 PFLOP/s, mxf4 199 us = 5.5, mxf8 432 us = 2.5 under the power cap. A K slab of a
+// pair takes 0.45 to 0.52 us in every format and at both widths, so neither its products (384 or 512 cycles) nor its 3, 6 or
+// 12 scale copies set that alone. 48060 x 1536 x 384 mxf8 with GELU into mxf8 74 us (43 us without GELU): the epilogue warps wait for
+// their own latencies, with half of the issue slots and 40 % of the FMA pipe in use; 1 x 4096 x 4096 mxf4 7 us, latency.
 #include "mx.cuh"
 #include "tc.cuh"
 
@@ -160,7 +161,7 @@ __device__ __forceinline__ void slab_products(uint32_t acc, uint32_t sfa, uint32
 // fit is off by 8e-8 at most and, so that a block of very negative sums keeps its scale and codes, by 8e-4 of what is left of
 // them down to -5.5 and 6e-3 beyond. From -13 on that is below f32's normal numbers and the exponential 0. Evaluated in f32:
 // rms 6.5e-8 on [-4, 4], 1.1e-7 beyond f32's own rounding at most. (A clamp at 5.5 and degree 7: rms 5.3e-8, but -1.04e-7
-// for every x below -5.5; 48060 x 1536 x 384 mxf8 -> mxf8 73.8 us with it, 74.5 us so. Degree 10: 77 us.) NaN stays NaN.
+// for every x below -5.5; 48060 x 1536 x 384 mxf8 -> mxf8 73 us with it, 74 us so. Degree 10: 77 us.) NaN stays NaN.
 // The coefficients lie in constant memory as pairs: as immediates each would cost the packed FMA two moves.
 __constant__ float2 kGelu[10] = {{-0.9999902248382568f, -0.9999902248382568f}, {-1.1512339115142822f, -1.1512339115142822f},
                                  {-0.45865750312805176f, -0.45865750312805176f}, {-0.05358625948429108f, -0.05358625948429108f},
@@ -185,7 +186,7 @@ __device__ __forceinline__ void gelu2(float& x0, float& x1) {
 // tanh(x) with a relative error below 1e-6 everywhere, since an output with block scales keeps small numbers' relative
 // precision: 1 - 2 / (e^2x + 1) from |x| = 0.5 on (its error of up to 4e-7 is absolute: at 1e-6 it would be a sixth of the
 // result), below it x + x^3 P(x^2), P of degree 3 fitted here to the least relative error (linear programming; 8e-8 in
-// f32's steps). 48060 x 1536 x 384 mxf8 -> bf16: 74 us, 64 us without the polynomial.
+// f32's steps). 48060 x 1536 x 384 mxf8 -> bf16: 72 us, 63 us without the polynomial.
 __constant__ float2 kTanh[4] = {{-0.333331435918808f, -0.333331435918808f}, {0.13325878977775574f, 0.13325878977775574f},
                                 {-0.05304549261927605f, -0.05304549261927605f}, {0.01724149100482464f, 0.01724149100482464f}};
 __device__ __forceinline__ void tanh2(float& x0, float& x1) {
@@ -234,7 +235,7 @@ __device__ __forceinline__ float array_scale(const Params& p, float& pre) {
 // act(acc * alpha + bias) + residual for columns c0 .. c0 + nv of a row (zeros behind them). `bias`: theirs, in shared
 // memory; with RES, `res` is the warp's residual buffer: its rows there (32 columns of f32, or 64 of 16 bits of which half
 // `half`), or with RES_ELEMENT room to exchange them. The arithmetic runs on packed pairs, one instruction for two
-// values: the epilogue is bound by instruction issue.
+// values: the epilogue's time goes by its instructions (three warps a scheduler, one instruction every seven cycles each).
 template <bool SCALED, bool RES>
 __device__ __forceinline__ void finish32(const Params& p, const float* bias, uint8_t* res, int half, int lane,
                                          int64_t row0, int c0, int nv, float alpha, const uint32_t (&r)[32], float (&v)[32]) {
