@@ -119,6 +119,69 @@ def test_rows_do_not_depend_on_one_another(fmt, m, n, k):
     assert torch.equal(mx.linear(x, w2, dtype=torch.float32)[:, c], y[:, c])
 
 
+def same_codes(q, last, first):
+    """The last rows of q, at a multiple of 128, and an array of those rows alone."""
+    assert first % 128 == 0
+    return torch.equal(q.data[first:], last.data) and torch.equal(q.scale_codes()[first:], last.scale_codes())
+
+
+def test_operands_beyond_32_bits():
+    """Rows of x, and of the stream of a norm, that begin beyond 2^32 bytes: against the same rows alone."""
+    m, k, first = 70000, 65504, 69888
+    x = torch.empty((m, k), dtype=torch.bfloat16, device="cuda")
+    x[:first] = 1
+    x[first:] = rows_of(m - first, k, torch.bfloat16, 3)
+    w = mx.quantize(rows_of(64, k, torch.float32, 4, 0), "mxf8")
+    q = mx.quantize(x, "mxf8")
+    last = mx.quantize(x[first:], "mxf8")
+    assert same_codes(q, last, first)
+    # The same kernel shape: 128 rows a tile, one CTA each.
+    rest = mx.quantize(x[first - 128 * 200:], "mxf8")
+    assert torch.equal(mx.linear(q, w, dtype=torch.float32)[first:], mx.linear(rest, w, dtype=torch.float32)[128 * 200:])
+    del q, rest
+    x, r = x[:, :32768], x[:, 32736:]  # rows 131008 bytes apart
+    q, s = mx.add_rms_norm(x, r)
+    one, t = mx.add_rms_norm(x[first:], r[first:])
+    assert torch.equal(s[first:], t) and same_codes(q, one, first)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 333, 1504])
+def test_gain_at_an_odd_address(fmt, dim):
+    x = rows_of(20, dim, torch.float32, 1)
+    gain = rows_of(1, dim + 3, torch.float32, 2, 0)[0]
+    for lo in range(4):
+        q, _ = mx.add_rms_norm(x, gain=gain[lo:lo + dim], format=fmt)
+        want, _ = mx.add_rms_norm(x, gain=gain[lo:lo + dim].clone(), format=fmt)
+        assert torch.equal(q.data, want.data) and torch.equal(q.scales, want.scales)
+
+
+def test_calls_from_several_threads():
+    """Threads with a stream each, in shapes of every kernel, get what one thread gets."""
+    import threading
+    shapes = [("mxf8", 3, 700, 2000), ("nvf4", 300, 520, 600), ("mxf4", 3000, 96, 300), ("mxf8", 133, 1544, 1000)]
+    work = [(*operands(f, m, n, k, m), rows_of(1, n, torch.float32, 9)[0]) for f, m, n, k in shapes]
+    want = [mx.linear(x, w, b, "gelu", format="mxf8") for x, w, b in work]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        x, w, b = work[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                y = mx.linear(x, w, b, "gelu", format="mxf8")
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(y.data, want[i].data) and torch.equal(y.scales, want[i].scales)):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(work))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 CAPTURE_FIRST = """
 import torch
 from ancha_b200 import microscaled as mx
