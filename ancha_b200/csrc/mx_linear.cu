@@ -960,8 +960,6 @@ split_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUt
     __syncwarp();
     if (*abort && threadIdx.x == 0) load_drain(full, STAGES, *issued);
     __syncwarp();
-    if (*abort && threadIdx.x == 0) load_drain(full, STAGES, *issued);
-    __syncwarp();
     cluster_sync();  // a CTA's shared memory stays while its peers read it
 }
 
